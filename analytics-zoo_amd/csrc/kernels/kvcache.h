@@ -1,0 +1,80 @@
+// Arguments of the paged key/value cache kernels (kvcache.hip), filled by the bindings.
+#pragma once
+#include <stdint.h>
+
+namespace zoo {
+
+constexpr int kKvMaxGroup = 256;        // query heads that may share one kv head
+constexpr int kKvMaxSlots = 1 << 30;    // slots one sequence may name
+
+// unsigned n / d for n < 2^31 as (mulhi(n, m) + n) >> s (Granlund and Montgomery's round-up method)
+struct FastDiv {
+  uint32_t d, m, s;
+};
+
+// element strides of a pool [pages, kv_heads, page, ...]
+struct PoolStride {
+  long page, head, row;
+};
+
+struct PagedAttnArgs {
+  const void* q;             // [B, H * G, D], strides q_b / q_h
+  const void* k;
+  const void* v;
+  const int* table;          // [B, width], row stride table_b
+  const int* len;            // [B]
+  const float* scores;       // pools [pages, H, page], or null: no weights wanted
+  float* scores_out;
+  void* o;                   // [B, H * G, D]
+  float* logits;             // [B, H, cap, G] raw products q.k (weights only)
+  float* part_o;             // [items, gs, D] partial sums of a split sequence
+  float* part_ml;            // [items, 16, 2] their running maximum (log2 units) and sum
+  long q_b, q_h, table_b;
+  PoolStride ks, vs, ss, sos;
+  FastDiv page;
+  int B, H, G, D, pages, cap;
+  int dtype;                 // 0 bf16, 1 fp16, 2 fp32
+  int gs;                    // min(G, 16)
+  int single;                // 1: every sequence is one work item (no join)
+  int target;                // chunks to aim at over the whole batch, per kv head block
+  float c;                   // scale * log2(e)
+};
+
+struct PagedAppendArgs {
+  const void* k;             // [B, T, H, D]
+  const void* v;
+  void* kp;
+  void* vp;
+  const int* table;
+  const int* len;
+  const int* counts;         // [B] or null: T tokens each
+  const int* seen;           // [B] or null: the position of a token is its slot
+  float* scores;             // pools or null
+  int* positions;
+  int* len_out;
+  long k_b, k_t, k_h, v_b, v_t, v_h, table_b;
+  PoolStride ks, vs, ss, ps;
+  FastDiv page, vec, heads;  // vec: 16-byte pieces of a row
+  int B, T, H, pages, cap, es;
+};
+
+struct PagedEvictArgs {
+  void* kp;
+  void* vp;
+  const float* scores;
+  const int* positions;
+  float* scores_out;
+  int* positions_out;
+  const int* table;
+  const int* len;
+  const int* seen;
+  int* len_out;
+  int* moves;                // [B, H, 2, most]: slots given up below the budget, and the kept ones that take them
+  int* count;                // [B, H] how many of each
+  long table_b;
+  PoolStride ks, vs, ss, ps, sos, pos;
+  FastDiv page, vec;
+  int B, H, pages, cap, es, budget, recent, most;
+};
+
+}  // namespace zoo

@@ -6,10 +6,13 @@
 // Kernels run on PyTorch's current HIP stream, so they order correctly with
 // any other torch work and are capturable into hipGraphs.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
 #include <hip/hip_runtime.h>
 
 #include "kernels/geom.h"
+#include "kernels/kvcache.h"
 #include "kernels/ncf.h"
 
 using zoo::ConvGeom;
@@ -199,6 +202,9 @@ hipError_t zoo_box_decode(const float*, const float*, float*, int, int, float, f
 hipError_t zoo_attn_bwd(const void*, const void*, const void*, const void*, const float*, const void*, const float*,
                         float*, void*, void*, void*, int, int, int, int, int, float, int, const long*, float, uint64_t,
                         hipStream_t);
+hipError_t zoo_paged_attn(const zoo::PagedAttnArgs*, int, hipStream_t);
+hipError_t zoo_paged_append(const zoo::PagedAppendArgs*, hipStream_t);
+hipError_t zoo_paged_evict(const zoo::PagedEvictArgs*, hipStream_t);
 }
 
 namespace {
@@ -3091,6 +3097,234 @@ void attn_bwd_strided(torch::Tensor dout, torch::Tensor q, torch::Tensor k, torc
 }
 
 
+// ---- paged key/value cache (kvcache.hip): pools [pages, kv_heads, page, D], page table [B, width] ----
+struct PagedCache {
+  int64_t P, H, page, D, B, width, cap;
+  int dtype;
+  int es;
+};
+
+zoo::FastDiv fast_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  return {d, (uint32_t)((((1ull << s) - d) << 32) / d + 1), s};
+}
+
+zoo::PoolStride pool_stride(const torch::Tensor& t) { return {(long)t.stride(0), (long)t.stride(1), (long)t.stride(2)}; }
+
+void req_rows(const torch::Tensor& t, const char* what) {
+  const int64_t n = 16 / (int64_t)t.element_size();
+  TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, what, ": the head dimension must be contiguous");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, what, ": must start on 16 bytes");
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    TORCH_CHECK(t.size(i) <= 1 || t.stride(i) % n == 0, what, ": rows must start on 16 bytes");
+}
+
+// slots that a row of the table may name (at most max_length of them, if that is given)
+PagedCache paged_check(const torch::Tensor& kp, const torch::Tensor& vp, const torch::Tensor& table,
+                       const torch::Tensor& lengths, c10::optional<int64_t> max_length, const char* what) {
+  PagedCache c;
+  TORCH_CHECK(kp.is_cuda() && kp.dim() == 4 && vp.dim() == 4, what, ": k_pages and v_pages must be [pages, kv_heads, page, dim]");
+  TORCH_CHECK(kp.sizes() == vp.sizes() && kp.scalar_type() == vp.scalar_type(), what, ": k_pages and v_pages differ");
+  switch (kp.scalar_type()) {
+    case at::kBFloat16: c.dtype = 0; break;
+    case at::kHalf: c.dtype = 1; break;
+    case at::kFloat: c.dtype = 2; break;
+    default: TORCH_CHECK(false, what, ": the cache must be bfloat16, float16 or float32");
+  }
+  c.es = (int)kp.element_size();
+  c.P = kp.size(0), c.H = kp.size(1), c.page = kp.size(2), c.D = kp.size(3);
+  TORCH_CHECK(c.D >= 8 && c.D <= 256 && c.D % 8 == 0, what, ": the head dimension must be a multiple of 8 up to 256");
+  TORCH_CHECK(c.H >= 1 && c.page >= 1 && c.page <= zoo::kKvMaxSlots, what, ": no kv heads or no rows in a page");
+  TORCH_CHECK(c.P < (1LL << 31), what, ": too many pages");
+  req_rows(kp, "k_pages");
+  req_rows(vp, "v_pages");
+  TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2, what, ": page_table must be int32 [batch, pages of a sequence]");
+  TORCH_CHECK(table.size(1) <= 1 || table.stride(1) == 1, what, ": page_table rows must be contiguous");
+  c.B = table.size(0), c.width = table.size(1);
+  TORCH_CHECK(lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.size(0) == c.B, what,
+              ": lengths must be int32 [batch]");
+  TORCH_CHECK(c.B <= 1 || lengths.stride(0) == 1, what, ": lengths must be contiguous");
+  TORCH_CHECK(c.width <= zoo::kKvMaxSlots / c.page, what, ": a sequence may have at most 2^30 slots");
+  c.cap = c.P == 0 ? 0 : c.width * c.page;
+  if (max_length.has_value()) {
+    TORCH_CHECK(*max_length >= 0, what, ": max_length must not be negative");
+    c.cap = std::min(c.cap, *max_length);
+  }
+  for (const torch::Tensor* t : {&vp, &table, &lengths})
+    TORCH_CHECK(t->device() == kp.device(), what, ": all tensors must be on one device");
+  return c;
+}
+
+void paged_side(const torch::Tensor& t, const torch::Tensor& kp, at::ScalarType dt, const char* name, const char* what) {
+  TORCH_CHECK(t.scalar_type() == dt && t.dim() == 3 && t.size(0) == kp.size(0) && t.size(1) == kp.size(1) &&
+                  t.size(2) == kp.size(2),
+              what, ": ", name, " must be ", dt, " [pages, kv_heads, page]");
+  TORCH_CHECK(t.device() == kp.device(), what, ": all tensors must be on one device");
+}
+
+void paged_ints(const torch::Tensor& t, const torch::Tensor& lengths, const char* name, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == lengths.size(0) &&
+                  (t.size(0) <= 1 || t.stride(0) == 1),
+              what, ": ", name, " must be int32 [batch], contiguous");
+  TORCH_CHECK(t.device() == lengths.device(), what, ": all tensors must be on one device");
+}
+
+// pools that are written must not overlap themselves or each other
+void paged_written(const torch::Tensor& kp, const torch::Tensor& vp) {
+  at::assert_no_internal_overlap(kp);
+  at::assert_no_internal_overlap(vp);
+  at::assert_no_partial_overlap(kp, vp);
+  TORCH_CHECK(at::get_overlap_status(kp, vp) != at::MemOverlapStatus::Full || kp.numel() == 0,
+              "k_pages and v_pages are the same memory");
+}
+
+torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor vp, torch::Tensor table,
+                              torch::Tensor lengths, double scale, c10::optional<torch::Tensor> scores,
+                              c10::optional<torch::Tensor> scores_out, c10::optional<int64_t> max_length) {
+  const char* what = "paged_attention";
+  const PagedCache c = paged_check(kp, vp, table, lengths, max_length, what);
+  c10::DeviceGuard guard(kp.device());
+  TORCH_CHECK(q.dim() == 3 && q.size(0) == c.B && q.size(2) == c.D && q.scalar_type() == kp.scalar_type() &&
+                  q.device() == kp.device(),
+              what, ": q must be [batch, heads, dim] of the cache's type and device");
+  req_rows(q, "q");
+  TORCH_CHECK(q.size(1) >= c.H && q.size(1) % c.H == 0, what, ": the heads of q must be a multiple of the cache's kv heads");
+  TORCH_CHECK(std::isfinite(scale), what, ": scale must be finite");
+  const int64_t G = q.size(1) / c.H, hbs = (G + 15) / 16;
+  TORCH_CHECK(G <= zoo::kKvMaxGroup, what, ": at most 256 query heads may share a kv head");
+  const bool weights = scores.has_value() && scores->defined();
+  TORCH_CHECK(weights || !scores_out.has_value(), what, ": scores_out without scores");
+  if (weights) {
+    paged_side(*scores, kp, at::kFloat, "scores", what);
+    if (!scores_out.has_value()) scores_out = scores;
+    paged_side(*scores_out, kp, at::kFloat, "scores_out", what);
+    at::assert_no_internal_overlap(*scores_out);
+    at::assert_no_partial_overlap(*scores_out, *scores);
+  }
+  auto o = torch::empty({c.B, c.H * G, c.D}, q.options());
+  if (o.numel() == 0) return o;
+  const int64_t per_seq = c.H * hbs;
+  // chunks to aim at: enough to fill the chip, and no longer than the mean sequence, so that one long
+  // sequence among short ones is shared out
+  static const int64_t cus = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int64_t target = std::max<int64_t>(c.B, (3 * cus + per_seq - 1) / per_seq);
+  zoo::PagedAttnArgs a{};
+  a.single = c.cap <= 256;
+  const int64_t items = (a.single ? c.B : c.B + target) * per_seq;
+  TORCH_CHECK(items < (1LL << 31), what, ": too many heads in the batch");
+  auto f32 = q.options().dtype(at::kFloat);
+  torch::Tensor ml, po, logits;
+  const int64_t gs = std::min<int64_t>(G, 16);
+  if (!a.single || weights) ml = torch::empty({items, 16, 2}, f32);
+  if (!a.single) po = torch::empty({items, gs, c.D}, f32);
+  if (weights) logits = torch::empty({c.B, c.H, c.cap, G}, f32);
+  a.q = q.data_ptr(), a.k = kp.data_ptr(), a.v = vp.data_ptr();
+  a.table = table.data_ptr<int>(), a.len = lengths.data_ptr<int>();
+  a.o = o.data_ptr();
+  if (weights) {
+    a.scores = scores->data_ptr<float>(), a.scores_out = scores_out->data_ptr<float>();
+    a.ss = pool_stride(*scores), a.sos = pool_stride(*scores_out);
+    a.logits = logits.data_ptr<float>();
+  }
+  a.part_ml = ml.defined() ? ml.data_ptr<float>() : nullptr;
+  a.part_o = po.defined() ? po.data_ptr<float>() : nullptr;
+  a.q_b = q.stride(0), a.q_h = q.stride(1), a.table_b = table.stride(0);
+  a.ks = pool_stride(kp), a.vs = pool_stride(vp);
+  a.page = fast_div((uint32_t)c.page);
+  a.B = c.B, a.H = c.H, a.G = G, a.D = c.D, a.pages = c.P, a.cap = c.cap, a.dtype = c.dtype, a.gs = gs;
+  a.target = target;
+  a.c = (float)(scale * 1.4426950408889634);
+  check_hip(zoo_paged_attn(&a, (int)items, cur_stream()), what);
+  return o;
+}
+
+torch::Tensor paged_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, torch::Tensor vp, torch::Tensor table,
+                           torch::Tensor lengths, c10::optional<torch::Tensor> counts, c10::optional<torch::Tensor> seen,
+                           c10::optional<torch::Tensor> scores, c10::optional<torch::Tensor> positions) {
+  const char* what = "paged_append";
+  const PagedCache c = paged_check(kp, vp, table, lengths, c10::nullopt, what);
+  c10::DeviceGuard guard(kp.device());
+  for (const torch::Tensor* t : {&k, &v}) {
+    TORCH_CHECK(t->dim() == 4 && t->size(0) == c.B && t->size(2) == c.H && t->size(3) == c.D &&
+                    t->scalar_type() == kp.scalar_type() && t->device() == kp.device(),
+                what, ": k and v must be [batch, tokens, kv_heads, dim] of the cache's type and device");
+    req_rows(*t, "k and v");
+  }
+  TORCH_CHECK(k.size(1) == v.size(1), what, ": k and v have other numbers of tokens");
+  const int64_t T = k.size(1), vec = c.D * c.es / 16;
+  TORCH_CHECK(T * c.H * vec < (1LL << 31) - 256 && c.B * ((T * c.H * vec + 255) / 256 + 1) < (1LL << 31), what,
+              ": too many tokens in one call");
+  paged_written(kp, vp);
+  if (counts.has_value()) paged_ints(*counts, lengths, "counts", what);
+  if (seen.has_value()) paged_ints(*seen, lengths, "seen", what);
+  if (scores.has_value()) {
+    paged_side(*scores, kp, at::kFloat, "scores", what);
+    at::assert_no_internal_overlap(*scores);
+  }
+  if (positions.has_value()) {
+    paged_side(*positions, kp, at::kInt, "positions", what);
+    at::assert_no_internal_overlap(*positions);
+  }
+  auto len_out = torch::empty({c.B}, lengths.options());
+  if (c.B == 0) return len_out;
+  zoo::PagedAppendArgs a{};
+  a.k = k.data_ptr(), a.v = v.data_ptr(), a.kp = kp.data_ptr(), a.vp = vp.data_ptr();
+  a.table = table.data_ptr<int>(), a.len = lengths.data_ptr<int>();
+  a.counts = opt_ptr<int>(counts), a.seen = opt_ptr<int>(seen);
+  a.scores = opt_ptr<float>(scores), a.positions = opt_ptr<int>(positions);
+  a.len_out = len_out.data_ptr<int>();
+  a.k_b = k.stride(0), a.k_t = k.stride(1), a.k_h = k.stride(2);
+  a.v_b = v.stride(0), a.v_t = v.stride(1), a.v_h = v.stride(2), a.table_b = table.stride(0);
+  a.ks = pool_stride(kp), a.vs = pool_stride(vp);
+  if (scores.has_value()) a.ss = pool_stride(*scores);
+  if (positions.has_value()) a.ps = pool_stride(*positions);
+  a.page = fast_div((uint32_t)c.page), a.vec = fast_div((uint32_t)vec), a.heads = fast_div((uint32_t)c.H);
+  a.B = c.B, a.T = T, a.H = c.H, a.pages = c.P, a.cap = c.cap, a.es = c.es;
+  check_hip(zoo_paged_append(&a, cur_stream()), what);
+  return len_out;
+}
+
+torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scores, torch::Tensor positions,
+                          torch::Tensor table, torch::Tensor lengths, torch::Tensor seen, int64_t budget, int64_t recent,
+                          torch::Tensor scores_out, torch::Tensor positions_out) {
+  const char* what = "paged_evict";
+  const PagedCache c = paged_check(kp, vp, table, lengths, c10::nullopt, what);
+  c10::DeviceGuard guard(kp.device());
+  TORCH_CHECK(budget >= 1 && budget <= zoo::kKvMaxSlots, what, ": budget must be from 1 to 2^30");
+  TORCH_CHECK(recent >= 0 && recent <= budget, what, ": recent must be from 0 to the budget");
+  paged_written(kp, vp);
+  paged_ints(seen, lengths, "seen", what);
+  for (const torch::Tensor* t : {&scores, &scores_out}) paged_side(*t, kp, at::kFloat, "scores", what);
+  for (const torch::Tensor* t : {&positions, &positions_out}) paged_side(*t, kp, at::kInt, "positions", what);
+  at::assert_no_internal_overlap(scores_out);
+  at::assert_no_internal_overlap(positions_out);
+  at::assert_no_partial_overlap(scores_out, scores);
+  at::assert_no_partial_overlap(positions_out, positions);
+  auto len_out = torch::empty({c.B}, lengths.options());
+  if (c.B == 0) return len_out;
+  const int64_t vec = c.D * c.es / 16, rows = c.B * c.H;
+  const int64_t most = std::max<int64_t>(0, std::min(budget, c.cap - budget));
+  TORCH_CHECK(rows * ((most * vec + 255) / 256 + 1) < (1LL << 31) && most * vec < (1LL << 31) - 256, what,
+              ": too many heads or slots in the batch");
+  auto moves = torch::empty({rows * (2 * most + 1)}, lengths.options());
+  zoo::PagedEvictArgs a{};
+  a.kp = kp.data_ptr(), a.vp = vp.data_ptr();
+  a.scores = scores.data_ptr<float>(), a.positions = positions.data_ptr<int>();
+  a.scores_out = scores_out.data_ptr<float>(), a.positions_out = positions_out.data_ptr<int>();
+  a.table = table.data_ptr<int>(), a.len = lengths.data_ptr<int>(), a.seen = seen.data_ptr<int>();
+  a.len_out = len_out.data_ptr<int>();
+  a.count = moves.data_ptr<int>(), a.moves = a.count + rows;
+  a.table_b = table.stride(0);
+  a.ks = pool_stride(kp), a.vs = pool_stride(vp), a.ss = pool_stride(scores), a.ps = pool_stride(positions);
+  a.sos = pool_stride(scores_out), a.pos = pool_stride(positions_out);
+  a.page = fast_div((uint32_t)c.page), a.vec = fast_div((uint32_t)vec);
+  a.B = c.B, a.H = c.H, a.pages = c.P, a.cap = c.cap, a.es = c.es;
+  a.budget = budget, a.recent = recent, a.most = most;
+  check_hip(zoo_paged_evict(&a, cur_stream()), what);
+  return len_out;
+}
+
 // ---- int8 quantized inference ----
 torch::Tensor absmax(torch::Tensor x) {
   TORCH_CHECK(x.is_cuda() && x.is_contiguous(), "absmax: contiguous GPU tensor");
@@ -3557,6 +3791,9 @@ PYBIND11_MODULE(_C, m) {
   m.def("attn_bwd", &attn_bwd, py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("mask"),
         py::arg("o"), py::arg("lse"), py::arg("causal"), py::arg("pdrop") = 0.0, py::arg("seed") = 0);
   m.def("attn_bwd_strided", &attn_bwd_strided);
+  m.def("paged_attention", &paged_attention);
+  m.def("paged_append", &paged_append);
+  m.def("paged_evict", &paged_evict);
   m.def("rnn_fwd", &rnn_fwd, py::arg("xw"), py::arg("u"), py::arg("h0"), py::arg("c0"), py::arg("cell"),
         py::arg("act"), py::arg("iact"), py::arg("save"), py::arg("bhn") = py::none());
   m.def("rnn_bwd", &rnn_bwd);

@@ -1,0 +1,412 @@
+"""The paged key/value cache (zoo.ops.kvcache, csrc/kernels/kvcache.hip) against its definition in 64 bits,
+written slot by slot here.
+
+Tolerances. The attention output is rounded once to the cache's type: half a step, eps / 2 of the value. Before
+that everything is float32: the products q.k over D dims and the sums over n slots. With logits |s| <= 20, a
+logit is off by at most 20 (D + 3) 2^-24 in the worst order of summation, about sqrt(D) of these in practice; a
+weight by twice that relative; the weights' two-part 16-bit split by 2^-16 (bfloat16) or 2^-21 (float16). So an
+output is off by at most eps / 2 |o| + (twice the split + 2^-24 * 40 * (D + 3)) * sum_j w_j |v_j|; gathered weights by
+2^-24 * 40 * (D + 3) times the weight plus half a step of the score.
+"""
+import math
+
+import pytest
+import torch
+
+from zoo.ops import paged_append, paged_attention, paged_evict
+
+GPU = pytest.mark.gpu
+BF, HF, FL = torch.bfloat16, torch.float16, torch.float32
+
+
+def make(B, H, G, D, page, lengths, dtype, dev, seed=0, order="phsd", spare=3, width=None, junk=float("nan")):
+    """A cache whose sequences own scattered pages; rows nobody uses hold `junk`."""
+    g = torch.Generator().manual_seed(seed)
+    own = [-(-n // page) for n in lengths]
+    width = max([1] + own) if width is None else width
+    P = sum(own) + spare
+    ids = torch.randperm(P, generator=g)
+    table = torch.full((B, width), -7, dtype=torch.int32)
+    k, v = (torch.full((P, H, page, D), junk) for _ in range(2))
+    at = 0
+    for b, n in enumerate(lengths):
+        for i in range(own[b]):
+            p = int(ids[at])
+            at += 1
+            table[b, i] = p
+            rows = min(page, n - i * page)
+            k[p, :, :rows] = torch.randn(H, rows, D, generator=g)
+            v[p, :, :rows] = torch.randn(H, rows, D, generator=g)
+    q = torch.randn(B, H * G, D, generator=g) * 1.5
+
+    def lay(t):
+        t = t.to(dtype)
+        if order == "pshd":      # [pages, page, heads, dim] in memory
+            t = t.transpose(1, 2).contiguous().transpose(1, 2)
+        return t.to(dev) if order == "phsd" else _keep(t, dev)
+
+    def _keep(t, dev):
+        if dev == "cpu":
+            return t
+        return t.transpose(1, 2).to(dev).transpose(1, 2)
+    return q.to(dtype).to(dev), lay(k), lay(v), table.to(dev), torch.tensor(lengths, dtype=torch.int32, device=dev)
+
+
+def define(q, k, v, table, lengths, scale=None):
+    """o, sum_j w_j |v_j| and the weights [B][H, n], in float64 on the CPU."""
+    q, k, v = (t.double().cpu() for t in (q, k, v))
+    B, Hq, D = q.shape
+    H, page = k.shape[1], k.shape[2]
+    scale = 1 / math.sqrt(D) if scale is None else scale
+    o, mag, ws = torch.zeros(B, Hq, D).double(), torch.zeros(B, Hq, D).double(), []
+    for b in range(B):
+        n = int(lengths[b])
+        slots = [(int(table[b, s // page]), s % page) for s in range(n)]
+        w_b = torch.zeros(H, n).double()
+        for h in range(H if n else 0):
+            kk = torch.stack([k[p, h, r] for p, r in slots])
+            vv = torch.stack([v[p, h, r] for p, r in slots])
+            for g in range(Hq // H):
+                i = h * (Hq // H) + g
+                w = torch.softmax(kk @ q[b, i] * scale, 0)
+                o[b, i] = w @ vv
+                mag[b, i] = w @ vv.abs()
+                w_b[h] += w
+        ws.append(w_b)
+    return o, mag, ws
+
+
+def close(o, ref, mag, D):
+    eps = torch.finfo(o.dtype).eps
+    split = {BF: 2.0 ** -15, HF: 2.0 ** -20, FL: 0.0}[o.dtype]
+    tol = eps / 2 * ref.abs() + (split + 2.0 ** -24 * 40 * (D + 3)) * mag + 1e-30
+    if o.dtype == HF:
+        tol = tol + 2.0 ** -25      # half a step of its subnormal numbers
+    err = (o.double().cpu() - ref).abs()
+    assert torch.isfinite(o.float()).all()
+    assert (err <= tol).all(), (err / tol).max().item()
+
+
+CASES = [
+    # H, G, D, page, dtype, order, lengths
+    (1, 1, 64, 16, BF, "phsd", [1]),
+    (12, 1, 64, 16, BF, "phsd", [77]),
+    (3, 1, 64, 64, BF, "pshd", [0, 1, 63, 64, 65, 200]),
+    (2, 4, 128, 16, BF, "phsd", [513, 0, 31, 32, 33, 129, 1]),
+    (2, 4, 128, 16, HF, "pshd", [513, 0, 31, 32, 33, 129, 1]),
+    (2, 8, 128, 64, FL, "phsd", [300, 17, 0, 16]),
+    (1, 16, 256, 32, BF, "phsd", [700, 5]),
+    (2, 3, 256, 32, FL, "phsd", [130, 5, 16]),
+    (1, 24, 64, 48, HF, "phsd", [900, 20]),          # two blocks of query heads
+    (2, 71, 64, 16, BF, "phsd", [100, 300]),         # five of them
+    (1, 2, 16, 24, BF, "phsd", [500, 3]),
+    (2, 1, 40, 7, BF, "phsd", [400, 0, 6, 7, 8]),    # no multiple of 16 in sight
+    (2, 5, 80, 1, HF, "phsd", [270, 4]),
+    (3, 2, 96, 100, FL, "pshd", [410, 99, 100, 101]),
+    (2, 2, 200, 33, BF, "phsd", [290, 64]),
+    (1, 1, 8, 5, FL, "phsd", [37]),
+    (1, 4, 128, 128, BF, "phsd", [5000]),            # split over many workgroups
+    (2, 2, 128, 20, HF, "phsd", [3000, 1, 0, 0, 40]),
+]
+
+
+def _check_attention(dev, H, G, D, page, dtype, order, lengths, weights):
+    q, k, v, table, n = make(len(lengths), H, G, D, page, lengths, dtype, dev, order=order)
+    ref, mag, ws = define(q, k, v, table, lengths)
+    if not weights:
+        close(paged_attention(q, k, v, table, n), ref, mag, D)
+        return
+    start = torch.rand(k.shape[:3]).to(dev)
+    out = torch.full_like(start, -3.0)
+    close(paged_attention(q, k, v, table, n, scores=start, scores_out=out), ref, mag, D)
+    want = torch.full(k.shape[:3], -3.0).double()     # slots behind the last keep what they held
+    tol = torch.zeros(k.shape[:3]).double()
+    for b, m in enumerate(lengths):
+        for s in range(m):
+            at = (int(table[b, s // page]), slice(None), s % page)
+            want[at] = start[at].double().cpu() + ws[b][:, s]
+            tol[at] = 2.0 ** -24 * 40 * (D + 3) * ws[b][:, s] + 2.0 ** -24 * want[at]
+    assert ((out.double().cpu() - want).abs() <= tol + 1e-30).all()
+    # in place: the same sums
+    paged_attention(q, k, v, table, n, scores=start)
+    used = want != -3.0
+    assert torch.equal(start.cpu()[used], out.cpu()[used])
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("H,G,D,page,dtype,order,lengths", CASES[:14])
+def test_attention_cpu(H, G, D, page, dtype, order, lengths, weights):
+    _check_attention("cpu", H, G, D, page, dtype, order, lengths, weights)
+
+
+@GPU
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("H,G,D,page,dtype,order,lengths", CASES)
+def test_attention_gpu(gpu, H, G, D, page, dtype, order, lengths, weights):
+    _check_attention("cuda", H, G, D, page, dtype, order, lengths, weights)
+
+
+# ---------------------------------------------------------------------------- values that arithmetic must not touch
+def _check_odd_values(dev, dtype=BF):
+    q, k, v, table, n = make(3, 2, 2, 64, 16, [40, 33, 20], dtype, dev)
+    # a key that makes one logit -inf: weight 0, and the others as if it were not there
+    p, r = int(table[0, 1]), 3
+    k[p, 0, r] = 0
+    k[p, 0, r, 5] = -math.inf
+    q[0, :2, 5] = 1.0
+    ref, mag, _ = define(q, k, v, table, [40, 33, 20])
+    assert torch.isfinite(ref[0, :2]).all()
+    o = paged_attention(q, k, v, table, n)
+    close(o, ref, mag, 64)
+    # an infinite value with weight comes through, a NaN key makes its heads NaN and no other
+    v[int(table[1, 0]), 1, 2, 7] = math.inf
+    k[int(table[2, 0]), 1, 4, 9] = math.nan
+    o = paged_attention(q, k, v, table, n).float().cpu()
+    assert o[1, 2, 7] == math.inf and o[1, 3, 7] == math.inf and torch.isfinite(o[1, :2]).all()
+    assert torch.isnan(o[2, 2:]).all() and torch.isfinite(o[2, :2]).all()
+    # huge logits: all weight on one slot
+    q2 = q * (1e4 if dtype != HF else 1e3)
+    ref, mag, _ = define(q2[:1, :2], k[:, :1], v[:, :1], table[:1], [40])
+    o = paged_attention(q2, k, v, table, n)
+    assert (o[0, :2].double().cpu() - ref[0]).abs().max() <= 2.0 ** -7 * ref.abs().max()
+
+
+def test_odd_values_cpu():
+    _check_odd_values("cpu")
+
+
+@GPU
+@pytest.mark.parametrize("dtype", [BF, HF, FL])
+def test_odd_values_gpu(gpu, dtype):
+    _check_odd_values("cuda", dtype)
+
+
+def _check_bad(dev):
+    """Lengths and pages that point nowhere: NaN for that sequence, nothing written, the others unharmed."""
+    lengths = [40, 33, 20, 70]
+    q, k, v, table, n = make(4, 2, 2, 64, 16, lengths, BF, dev)
+    good = paged_attention(q, k, v, table, n)
+    for what in ("page", "negative page", "long", "negative"):
+        t2, n2 = table.clone(), n.clone()
+        if what == "page":
+            t2[1, 2] = k.shape[0]
+        elif what == "negative page":
+            t2[1, 0] = -1
+        else:
+            n2[1] = 16 * table.shape[1] + 1 if what == "long" else -1
+        o = paged_attention(q, k, v, t2, n2)
+        assert torch.isnan(o[1]).all(), what
+        assert torch.equal(o[[0, 2, 3]], good[[0, 2, 3]]), what
+        pools = [k.clone(), v.clone(), torch.rand(k.shape[:3]).to(dev), torch.randint(0, 70, k.shape[:3]).int().to(dev)]
+        before = [x.clone() for x in pools]
+        kk = torch.randn(4, 1, 2, 64).to(BF).to(dev)
+        if what in ("long", "negative"):
+            new = paged_append(kk[1:2], kk[1:2], pools[0], pools[1], t2[1:2], n2[1:2], scores=pools[2], positions=pools[3])
+            assert torch.equal(new, n2[1:2])
+        else:
+            n3 = torch.tensor([32 if what == "page" else 0], dtype=torch.int32, device=dev)
+            new = paged_append(kk[1:2], kk[1:2], pools[0], pools[1], t2[1:2], n3, scores=pools[2], positions=pools[3])
+            assert torch.equal(new, n3 + 1)
+        new = paged_evict(*pools, t2[1:2], n2[1:2], n2[1:2].clone(), 10, 2)
+        assert torch.equal(new, n2[1:2])
+        for x, y in zip(pools, before):
+            assert torch.equal(x.nan_to_num(), y.nan_to_num()), what
+    # longer than the bound that the caller gave
+    o = paged_attention(q, k, v, table, n, max_length=40)
+    assert torch.isnan(o[3]).all() and torch.equal(o[:3], good[:3])
+
+
+def test_bad_lengths_and_pages_cpu():
+    _check_bad("cpu")
+
+
+@GPU
+def test_bad_lengths_and_pages_gpu(gpu):
+    _check_bad("cuda")
+
+
+@GPU
+def test_append_past_the_table_gpu(gpu):
+    _past_the_table("cuda")
+
+
+def test_append_past_the_table_cpu():
+    _past_the_table("cpu")
+
+
+def _past_the_table(dev):
+    q, k, v, table, n = make(2, 1, 1, 8, 4, [6, 3], FL, dev, width=2)
+    table[1, 1] = int(k.shape[0]) - 1 if int(k.shape[0]) - 1 not in table.tolist()[0] + table.tolist()[1] else _free(table, k)
+    new_k, new_v = torch.randn(2, 1, 2, 5, 1, 8).to(dev)[:, 0]
+    k0 = k.clone()
+    new = paged_append(new_k, new_v, k, v, table, n)
+    assert new.tolist() == [11, 8]
+    written = {(int(table[0, 1]), 2): (0, 0), (int(table[0, 1]), 3): (0, 1)}
+    for t in range(5):
+        written[(int(table[1, (3 + t) // 4]), (3 + t) % 4)] = (1, t)
+    for p in range(k.shape[0]):
+        for r in range(4):
+            src = written.get((p, r))
+            want = k0[p, :, r] if src is None else new_k[src[0], src[1]]
+            assert torch.equal(k[p, :, r].nan_to_num(), want.nan_to_num())
+    assert torch.isnan(paged_attention(q, k, v, table, new)[0]).all()
+
+
+def _free(table, k):
+    return next(p for p in range(k.shape[0]) if p not in set(table.flatten().tolist()))
+
+
+# ---------------------------------------------------------------------------- append
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("H,D,page,T,dtype,order,counted", [
+    (12, 64, 16, 1, BF, "phsd", False), (2, 128, 64, 33, HF, "pshd", True), (3, 8, 7, 20, FL, "phsd", True),
+    (1, 256, 1, 5, FL, "pshd", True), (5, 40, 24, 100, BF, "phsd", True), (2, 16, 16, 0, BF, "phsd", False)])
+def test_append(dev, H, D, page, T, dtype, order, counted):
+    lengths = [0, 5, page, 2 * page - 1, 31]
+    counts = [T, 0, max(T - 1, 0), min(1, T), T + 9] if counted else [T] * 5       # more than there are: all of them
+    real = [max(0, min(T, c)) for c in counts]
+    q, k, v, table, _ = make(5, H, 1, D, page, [a + b for a, b in zip(lengths, real)], dtype, dev, order=order, junk=2.0)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    seen = n + 100
+    qkv = torch.randn(5, T, 3, H, D).to(dtype).to(dev)
+    new_k, new_v = qkv[:, :, 1], qkv[:, :, 2]
+    scores, positions = torch.rand(k.shape[:3]).to(dev), torch.zeros(k.shape[:3]).int().to(dev)
+    want = [t.clone() for t in (k, v, scores, positions)]
+    for b in range(5):
+        for t in range(real[b]):
+            s = lengths[b] + t
+            at = (int(table[b, s // page]), slice(None), s % page)
+            want[0][at], want[1][at], want[2][at], want[3][at] = new_k[b, t], new_v[b, t], 0.0, lengths[b] + 100 + t
+    c = torch.tensor(counts, dtype=torch.int32, device=dev) if counted else None
+    got = paged_append(new_k, new_v, k, v, table, n, counts=c, seen=seen, scores=scores, positions=positions)
+    assert got.tolist() == [a + b for a, b in zip(lengths, real)]
+    assert n.tolist() == lengths
+    for x, y in zip((k, v, scores, positions), want):
+        assert torch.equal(x, y)
+    positions.zero_()
+    paged_append(new_k, new_v, k, v, table, n, counts=c, positions=positions)       # by default the slot is the position
+    for b in range(5):
+        for t in range(real[b]):
+            s = lengths[b] + t
+            assert (positions[int(table[b, s // page]), :, s % page] == s).all()
+
+
+# ---------------------------------------------------------------------------- evict
+def evict_by_definition(pools, table, lengths, seen, budget, recent):
+    k, v, scores, positions = (t.clone() for t in pools)
+    H, page = k.shape[1], k.shape[2]
+    sc, po = scores.cpu(), positions.cpu()
+    for b, n in enumerate(lengths):
+        at = [(int(table[b, s // page]), s % page) for s in range(n)]
+        for h in range(H if n > budget else 0):
+            rank = []
+            for s, (p, r) in enumerate(at):
+                x = float(sc[p, h, r])
+                late = int(po[p, h, r]) >= seen[b] - recent
+                rank.append((0 if late else 2 if math.isnan(x) else 1, 0.0 if late or math.isnan(x) else -x, s))
+            kept = {s for _, _, s in sorted(rank)[:budget]}
+            holes = [s for s in range(budget) if s not in kept]
+            behind = [s for s in sorted(kept) if s >= budget]
+            for d, s in zip(holes, behind):
+                for t in (k, v, scores, positions):
+                    t[at[d][0], h, at[d][1]] = t[at[s][0], h, at[s][1]]
+    return k, v, scores, positions
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("H,D,page,dtype,order,lengths,budget,recent,kind", [
+    (2, 64, 16, BF, "phsd", [100, 0, 50, 51, 1], 50, 10, "plain"),
+    (1, 8, 7, FL, "pshd", [60, 20, 13], 1, 0, "plain"),
+    (3, 40, 24, HF, "phsd", [400, 399, 25], 24, 24, "ties"),
+    (2, 64, 1, BF, "phsd", [70, 64], 63, 1, "odd"),
+    (2, 128, 64, BF, "pshd", [513, 514, 512], 512, 128, "plain"),
+    (2, 16, 33, FL, "phsd", [1500, 1100, 1025], 700, 5, "ties"),
+    (1, 8, 128, BF, "phsd", [2500], 2048, 0, "zeros"),
+    (2, 8, 16, FL, "phsd", [300], 100, 50, "twice"),
+    (1, 8, 16, FL, "phsd", [30], 1000, 3, "plain"),
+])
+def test_evict(dev, H, D, page, dtype, order, lengths, budget, recent, kind):
+    B = len(lengths)
+    _, k, v, table, n = make(B, H, 1, D, page, lengths, dtype, dev, order=order, junk=2.0)
+    g = torch.Generator().manual_seed(5)
+    shape = k.shape[:3]
+    scores = torch.rand(shape, generator=g)
+    if kind == "ties":
+        scores = (scores * 4).floor() / 4
+    elif kind == "zeros":
+        scores.zero_()
+    elif kind == "odd":
+        special = torch.tensor([math.nan, math.inf, -math.inf, 0.0, -0.0, 1e-42, -1e-42, -3.0])
+        scores = special[torch.randint(0, 8, shape, generator=g)]
+    positions = torch.zeros(shape, dtype=torch.int32)
+    for b, m in enumerate(lengths):
+        for h in range(H):
+            order_ = torch.randperm(m, generator=g) if kind != "twice" else torch.randint(0, m, (m,), generator=g)
+            for s in range(m):
+                positions[int(table[b, s // page]), h, s % page] = int(order_[s])
+    scores, positions = scores.to(dev), positions.to(dev)
+    seen = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    want = evict_by_definition((k, v, scores, positions), table, lengths, lengths, budget, recent)
+    # out of place: scores and positions of the kept slots in new pools, nothing else there
+    k2, v2 = k.clone(), v.clone()
+    so, po = torch.full_like(scores, -5.0), torch.full_like(positions, -5)
+    got = paged_evict(k2, v2, scores, positions, table, n, seen, budget, recent, scores_out=so, positions_out=po)
+    assert got.tolist() == [min(m, budget) for m in lengths] and n.tolist() == lengths
+    assert torch.equal(k2, want[0]) and torch.equal(v2, want[1])
+    used = torch.zeros(shape, dtype=torch.bool)
+    for b, m in enumerate(lengths):
+        for s in range(min(m, budget)):
+            used[int(table[b, s // page]), :, s % page] = True
+    used = used.to(dev)
+    assert torch.equal(so[used].view(torch.int32), want[2][used].view(torch.int32)) and torch.equal(po[used], want[3][used])
+    assert (so[~used] == -5.0).all() and (po[~used] == -5).all()
+    # in place
+    got = paged_evict(k, v, scores, positions, table, n, seen, budget, recent)
+    assert got.tolist() == [min(m, budget) for m in lengths]
+    for x, y in zip((k, v, scores, positions), want):
+        assert torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
+
+
+# ---------------------------------------------------------------------------- refusals
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+def test_refusals(dev):
+    q, k, v, table, n = make(2, 2, 2, 16, 8, [9, 5], BF, dev)
+    s, p = torch.zeros(k.shape[:3]).to(dev), torch.zeros(k.shape[:3]).int().to(dev)
+    x = torch.zeros(2, 1, 2, 16).to(BF).to(dev)
+
+    def no(f, *a, **kw):
+        with pytest.raises((RuntimeError, TypeError)):
+            f(*a, **kw)
+    no(paged_attention, q[:, :3], k, v, table, n)
+    no(paged_attention, q[:1], k, v, table, n)
+    no(paged_attention, q[:, :, :8], k, v, table, n)
+    no(paged_attention, q, k, v[:, :1], table, n)
+    no(paged_attention, q, k, v, table.long(), n)
+    no(paged_attention, q, k, v, table, n.long())
+    no(paged_attention, q, k, v, table, n[:1])
+    no(paged_attention, q, k, v, table, n, scale=math.inf)
+    no(paged_attention, q, k, v, table, n, scores_out=s)
+    no(paged_attention, q, k, v, table, n, max_length=-1)
+    no(paged_attention, q.float().requires_grad_(), k.float(), v.float(), table, n)
+    no(paged_append, x[:1], x[:1], k, v, table, n)
+    no(paged_append, x[..., :8], x[..., :8], k, v, table, n)
+    no(paged_append, x.float(), x.float(), k, v, table, n)
+    no(paged_evict, k, v, s, p, table, n, n, 0)
+    no(paged_evict, k, v, s, p, table, n, n, 4, 5)
+    no(paged_evict, k, v, s, p, table, n, n, 4, -1)
+    if dev == "cuda":
+        no(paged_attention, q.half(), k, v, table, n)
+        no(paged_attention, q, k, v, table.cpu(), n)
+        no(paged_attention, q, k, v, table, n, scores=s[:1])
+        no(paged_attention, q, k, v, table, n, scores=s.double())
+        no(paged_attention, q, k, v, table, n, scores=s, scores_out=s.expand(4, *s.shape)[0, :1])
+        no(paged_attention, q, k.transpose(2, 3).contiguous().transpose(2, 3), v, table, n)
+        no(paged_attention, q[..., :12].contiguous(), k[..., :12].contiguous(), v[..., :12].contiguous(), table, n)
+        big = torch.zeros(3, 1, 8, 264, dtype=BF, device=dev)
+        no(paged_attention, big[:2, 0, :1], big, big, table, n)
+        wide = torch.zeros(2, 514, 16, dtype=BF, device=dev)
+        no(paged_attention, wide, k, v, table, n)                       # 257 heads to a kv head
+        no(paged_append, x, x, k, k, table, n)                          # keys and values in one place
+        no(paged_append, x, x, k[:1].expand(k.shape), v, table, n)
+        no(paged_evict, k, v, s.half(), p, table, n, n, 4)
+        no(paged_evict, k, v, s, p.long(), table, n, n, 4)
