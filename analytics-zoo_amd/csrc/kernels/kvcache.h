@@ -1,11 +1,13 @@
 // Arguments of the paged key/value cache kernels (kvcache.hip), filled by the bindings.
 #pragma once
+#include <hip/hip_runtime.h>
 #include <stdint.h>
 
 namespace zoo {
 
 constexpr int kKvMaxGroup = 256;        // query heads that may share one kv head
 constexpr int kKvMaxSlots = 1 << 30;    // slots one sequence may name
+constexpr int kEvictRow = 16 + 3 * 2048;  // ints of a row's selection state where it is shared out
 
 // unsigned n / d for n < 2^31 as (mulhi(n, m) + n) >> s (Granlund and Montgomery's round-up method)
 struct FastDiv {
@@ -29,14 +31,18 @@ struct PagedAttnArgs {
   float* logits;             // [B, H, cap, G] raw products q.k (weights only)
   float* part_o;             // [items, gs, D] partial sums of a split sequence
   float* part_ml;            // [items, 16, 2] their running maximum (log2 units) and sum
+  int4* plan;                // [items, 2] who does what, for the join; null where there is none
   long q_b, q_h, table_b;
   PoolStride ks, vs, ss, sos;
   FastDiv page;
   int B, H, G, D, pages, cap;
   int dtype;                 // 0 bf16, 1 fp16, 2 fp32
   int gs;                    // min(G, 16)
-  int single;                // 1: every sequence is one work item (no join)
-  int target;                // chunks to aim at over the whole batch, per kv head block
+  int single;                // 1: every sequence is one work item
+  int hbs;                   // blocks of 16 query heads per kv head
+  FastDiv step;              // H * hbs: items from one chunk to the next
+  float per_target;          // 0.999 / target: the chunks to aim at over the batch, per head block
+  int at_once;               // chunks per head block that the chip can run at once, 0: fewer than B
   float c;                   // scale * log2(e)
 };
 
@@ -71,10 +77,13 @@ struct PagedEvictArgs {
   int* len_out;
   int* moves;                // [B, H, 2, most]: slots given up below the budget, and the kept ones that take them
   int* count;                // [B, H] how many of each
+  int* hist;                 // rows shared out: [B * H, kEvictRow] zeroed, then [B * H, segs * 4] Counts
+  int* keys;                 // rows shared out: [B * H, cap]
   long table_b;
   PoolStride ks, vs, ss, ps, sos, pos;
   FastDiv page, vec;
   int B, H, pages, cap, es, budget, recent, most;
+  int segs;                  // workgroups to a row, 0: one, its keys in LDS
 };
 
 }  // namespace zoo

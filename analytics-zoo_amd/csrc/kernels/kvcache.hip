@@ -53,68 +53,122 @@ ZOO_DEV int seq_len(const int* len, int b, int cap) {
 
 ZOO_DEV int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// inclusive prefix sum over the wave: shifts within rows of 16 lanes, then each row's total to the ones behind it
+#define ZOO_DPP(x, ctrl, rows) __builtin_amdgcn_update_dpp(0, (x), ctrl, rows, 0xf, false)
+ZOO_DEV int wave_prefix(int x) {
+  x += ZOO_DPP(x, 0x111, 0xf);
+  x += ZOO_DPP(x, 0x112, 0xf);
+  x += ZOO_DPP(x, 0x114, 0xf);
+  x += ZOO_DPP(x, 0x118, 0xf);
+  x += ZOO_DPP(x, 0x142, 0xa);
+  x += ZOO_DPP(x, 0x143, 0xc);
+  return x;
+}
+ZOO_DEV float wave_total(float x) {
+  x += __int_as_float(ZOO_DPP(__float_as_int(x), 0x111, 0xf));
+  x += __int_as_float(ZOO_DPP(__float_as_int(x), 0x112, 0xf));
+  x += __int_as_float(ZOO_DPP(__float_as_int(x), 0x114, 0xf));
+  x += __int_as_float(ZOO_DPP(__float_as_int(x), 0x118, 0xf));
+  x += __int_as_float(ZOO_DPP(__float_as_int(x), 0x142, 0xa));
+  x += __int_as_float(ZOO_DPP(__float_as_int(x), 0x143, 0xc));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+#undef ZOO_DPP
+
 struct Work {
   int b, hk, hb;    // sequence, kv head, block of 16 query heads
   int chunk, n;     // which of the sequence's n chunks
   int s0, s1;       // its slots
   int len;          // the sequence's slots, -1: bad
   int first;        // item of the sequence's chunk 0, same head block
-  int step;         // items from one chunk to the next
 };
 
+ZOO_DEV int chunks_of(int len, int size) { return len <= size ? 1 : (int)(((unsigned)len + size - 1) / (unsigned)size); }
+
+// `want` slots rounded up to grains (a power of two), at least one; a sequence has 2^30 slots at most
+ZOO_DEV int chunk_size(float want, int grain) {
+  return max((int)ceilf(fminf(want, 0x1p30f) / grain), 1) * grain;
+}
+
 // Cuts the batch into chunks of `size` slots, a multiple of `grain`, such that there are at most
-// target + B of them per head block, and finds the chunk of this workgroup; every wave does so alone.
-// Every sequence has a chunk, if an empty one. Returns false for the items that are not needed.
+// target (1 + 1 / 512) + B of them per head block, and finds the chunk of this workgroup; every wave does so alone.
+// Every sequence has a chunk, if an empty one. False for the items that are not needed.
+// The logical item of this workgroup. Blocks of query heads of one kv head read the same keys and values: they are
+// put 8 workgroups apart, on one XCD, so that its L2 serves all but the first (there are 8 XCDs, and
+// workgroups go to them in turn).
+ZOO_DEV int item_of(const PagedAttnArgs& a) {
+  const int x = blockIdx.x;
+  if (a.hbs == 1) return x;
+  const int group = 8 * a.hbs, g = x / group, in = x - g * group;
+  return (g + 1) * group <= (int)gridDim.x ? g * group + (in & 7) * a.hbs + (in >> 3) : x;
+}
+
 ZOO_DEV bool find_work(const PagedAttnArgs& a, int grain, Work& w) {
   const int lane = threadIdx.x & 63;
-  const int hbs = (a.G + 15) >> 4, step = a.H * hbs;
-  const int t = blockIdx.x / step, hh = blockIdx.x - t * step;
-  w.hk = hh / hbs;
-  w.hb = hh - w.hk * hbs;
-  w.step = step;
-  int at = 0, size = kKvMaxSlots;
-  if (!a.single) {
-    long total = 0;
-    for (int b = lane; b < a.B; b += 64) total += max(seq_len(a.len, b, a.cap), 0);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-    // a chunk is at least one grain and at most a whole sequence, so this fits an int
-    const long want = (total + a.target - 1) / a.target;
-    size = (int)min((long)kKvMaxSlots, max((want + grain - 1) / grain, 1L) * grain);
+  const int item = item_of(a);
+  const int t = fdiv(item, a.step), hh = item - t * a.step.d;
+  w.hb = 0, w.hk = hh;
+  if (a.hbs > 1) w.hk = hh / a.hbs, w.hb = hh - w.hk * a.hbs;
+  if (a.single) {
+    w.b = t, w.chunk = 0, w.n = 1, w.first = item;
+    w.len = uni(seq_len(a.len, t, a.cap));
+    w.s0 = 0, w.s1 = w.len;
+    return true;
   }
-  int b = 0, chunk = 0, n = 0, len = 0;
-  bool found = false;
-  for (int b0 = 0; b0 < a.B && !found; b0 += 64) {
-    const int mine = b0 + lane < a.B ? seq_len(a.len, b0 + lane, a.cap) : 0;
-    const int chunks = b0 + lane < a.B ? max((max(mine, 0) + size - 1) / size, 1) : 0;
-    int upto = chunks;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += x;
+  const int mine0 = lane < a.B ? seq_len(a.len, lane, a.cap) : 0;
+  float total = (float)max(mine0, 0);
+  for (int b = lane + 64; b < a.B; b += 64) total += (float)max(seq_len(a.len, b, a.cap), 0);
+  total = wave_total(total);
+  // per_target is 0.999 / target, so that a total that divides evenly is not rounded up to another grain
+  int size = chunk_size(total * a.per_target, grain);
+  // Sequences end inside chunks, so there are more chunks than the total asks for: if they would
+  // not all run at once, longer ones (twice, as this is a fixed point's iteration).
+  for (int i = 0; i < 2 && a.at_once > 0; ++i) {
+    int n = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const int mine = b0 == 0 ? mine0 : b0 + lane < a.B ? seq_len(a.len, b0 + lane, a.cap) : 0;
+      n += __builtin_amdgcn_readlane(wave_prefix(b0 + lane < a.B ? chunks_of(mine, size) : 0), 63);
     }
+    if (n <= a.at_once) break;
+    size = chunk_size((float)size * n / a.at_once, grain);
+  }
+  int at = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int mine = b0 == 0 ? mine0 : b0 + lane < a.B ? seq_len(a.len, b0 + lane, a.cap) : 0;
+    const int chunks = b0 + lane < a.B ? chunks_of(mine, size) : 0;
+    const int upto = wave_prefix(chunks);
     const unsigned long long hit = __ballot(at + upto > t);
     if (hit) {
       const int who = __ffsll(hit) - 1;
-      b = b0 + who;
-      n = __shfl(chunks, who, 64);
-      len = __shfl(mine, who, 64);
-      at += __shfl(upto, who, 64) - n;
-      chunk = t - at;
-      found = true;
-    } else {
-      at += __shfl(upto, 63, 64);
+      w.b = b0 + who;
+      w.n = __builtin_amdgcn_readlane(chunks, who);
+      w.len = __builtin_amdgcn_readlane(mine, who);
+      at += __builtin_amdgcn_readlane(upto, who) - w.n;
+      w.chunk = t - at;
+      w.first = at * (int)a.step.d + hh;
+      w.s0 = w.chunk * size;
+      w.s1 = min(w.len, w.s0 + size);
+      return true;
     }
+    at += __builtin_amdgcn_readlane(upto, 63);
   }
-  if (!found) return false;
-  w.b = uni(b);
-  w.chunk = uni(chunk);
-  w.n = uni(n);
-  w.len = uni(len);
-  w.first = uni(at) * step + hh;
-  w.s0 = w.chunk * size;
-  w.s1 = min(w.len, w.s0 + size);
-  return true;
+  return false;
+}
+
+// what find_work found, for the join kernel: n = 0 where there is nothing
+ZOO_DEV void put_work(const PagedAttnArgs& a, const Work& w, bool found) {
+  if (a.plan != nullptr && threadIdx.x == 0) {
+    a.plan[2 * item_of(a)] = make_int4(w.b, w.chunk, found ? w.n : 0, w.len);
+    a.plan[2 * item_of(a) + 1] = make_int4(w.s0, w.s1, w.first, 0);
+  }
+}
+ZOO_DEV bool get_work(const PagedAttnArgs& a, Work& w) {
+  const int4 x = a.plan[2 * blockIdx.x], y = a.plan[2 * blockIdx.x + 1];
+  w.b = uni(x.x), w.chunk = uni(x.y), w.n = uni(x.z), w.len = uni(x.w);
+  w.s0 = uni(y.x), w.s1 = uni(y.y), w.first = uni(y.z);
+  const int hh = blockIdx.x - fdiv(blockIdx.x, a.step) * a.step.d;
+  w.hk = hh / a.hbs, w.hb = hh - w.hk * a.hbs;
+  return w.n > 0;
 }
 
 template <int DT, int DP>
@@ -178,16 +232,64 @@ ZOO_DEV void store_any(int dt, void* o, long at, float x) {
     store_out<kF32>(o, at, x);
 }
 
+// scores_out = scores + sum_g 2^(c x_g - lse_g) for the slots s0 .. s1 of one kv head, x the stored products
+// of its heads with the slot. A thread has several slots under way at a time: each is a chain of three loads.
+ZOO_DEV void gather_weights(const PagedAttnArgs& a, int b, int hk, int s0, int s1, const float* lse) {
+  const int* table = a.table + (long)b * a.table_b;
+  const float* logit = a.logits + ((long)b * a.H + hk) * a.cap * a.G;
+  constexpr int U = 4;
+  const int G = a.G, step = blockDim.x;
+  const float* in = a.scores + (long)hk * a.ss.head;
+  float* out = a.scores_out + (long)hk * a.sos.head;
+  for (int s = s0 + threadIdx.x; s < s1; s += U * step) {
+    int p[U];
+    float sum[U], was[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) p[u] = table[fdiv(min(s + u * step, s1 - 1), a.page)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = min(s + u * step, s1 - 1);
+      if ((unsigned)p[u] >= (unsigned)a.pages || s + u * step >= s1) p[u] = -1;
+      was[u] = p[u] < 0 ? 0.f : in[p[u] * a.ss.page + (long)(at - fdiv(at, a.page) * a.page.d) * a.ss.row];
+      sum[u] = 0.f;
+    }
+    if (G % 4 == 0) {
+      for (int g = 0; g < G; g += 4) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const f32x4 x = *(const f32x4*)(logit + (long)min(s + u * step, s1 - 1) * G + g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[u] += pow2(fmaf(x[i], a.c, -lse[g + i]));
+        }
+      }
+    } else {
+      for (int g = 0; g < G; ++g) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) sum[u] += pow2(fmaf(logit[(long)min(s + u * step, s1 - 1) * G + g], a.c, -lse[g]));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p[u] >= 0) {
+        const int at = s + u * step;
+        out[p[u] * a.sos.page + (long)(at - fdiv(at, a.page) * a.page.d) * a.sos.row] = was[u] + sum[u];
+      }
+  }
+}
+
 // DP: the head width rounded up; PAD: it was rounded; P16: pages of a multiple of 16 rows, so that a
 // 16-slot subtile lies in one page and its address is wave-uniform. Other page sizes look up a page per
 // slot.
 template <int DT, int DP, bool PAD, bool P16>
-__global__ __launch_bounds__(256) void paged_attn_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(256, DP == 256 ? (DT == kF32 ? 1 : 2) : DT == kF32 && DP == 128 && PAD ? 2 : 3) void paged_attn_kernel(const PagedAttnArgs a) {
   using T = Tile<DT, DP>;
   constexpr int NS = T::NS, KL = T::KL, VC = T::VC, VW = T::VW, VE = T::VE, NA = T::NA, ES = T::ES;
   extern __shared__ float lds[];  // [4][gb][DP + 4] sums, then [4][16][2] maximum and sum
+  __shared__ float lse[16];
   Work w;
-  if (!find_work(a, T::GRAIN, w)) return;
+  const bool found = find_work(a, T::GRAIN, w);
+  put_work(a, w, found);
+  if (!found) return;
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   const int row = lane & 15, quad = lane >> 4;
   const int gb = min(16, a.G - 16 * w.hb), D = a.D;
@@ -439,90 +541,89 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(const PagedAttnArgs a) 
       if (w.n == 1)
         store_out<DT>(a.o, out0 + (long)g * D + d, o / sum);
       else
-        a.part_o[((long)blockIdx.x * a.gs + g) * D + d] = o;
+        a.part_o[((long)item_of(a) * a.gs + g) * D + d] = o;
     }
-    if (d == 0 && a.part_ml != nullptr) {
-      a.part_ml[((long)blockIdx.x * 16 + g) * 2] = top;
-      a.part_ml[((long)blockIdx.x * 16 + g) * 2 + 1] = sum;
+    if (d == 0) {
+      if (a.part_ml != nullptr) {
+        a.part_ml[((long)item_of(a) * 16 + g) * 2] = top;
+        a.part_ml[((long)item_of(a) * 16 + g) * 2 + 1] = sum;
+      }
+      lse[g] = top + log2f(sum) - kUp;
     }
+  }
+  if (w.n == 1 && a.logits != nullptr && a.G <= 16) {
+    __syncthreads();    // orders the waves' products, which this workgroup reads back, as well
+    gather_weights(a, w.b, w.hk, w.s0, w.s1, lse);
   }
 }
 
+// folds the running maximum and sum (m2, l2), and what is weighted with them, into (m, l)
+ZOO_DEV void merge(float& m, float& l, float& x, float m2, float l2, float x2) {
+  const float top = fmaxf(m, m2), mu = top == -INFINITY ? 0.f : top;
+  const float f = pow2(m - mu), f2 = pow2(m2 - mu);
+  l = l * f + l2 * f2;
+  x = x * f + x2 * f2;
+  m = top;
+}
+
 // Joins the chunks of a sequence: chunk c of n writes the c-th part of the outputs, and the gathered
-// weights of its own slots.
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(const PagedAttnArgs a, int grain) {
-  __shared__ float lse[kKvMaxGroup], part[256];
+// weights of its own slots. Bound by the latency of its chain of loads, not by bytes: so every thread
+// takes the maxima and sums along with the partial outputs instead of waiting for their total first.
+constexpr int kJoinThreads = 512;
+
+__global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const PagedAttnArgs a) {
+  __shared__ float lse[kKvMaxGroup], sm[kJoinThreads], sl[kJoinThreads], sx[kJoinThreads];
   Work w;
-  if (!find_work(a, grain, w)) return;
-  const bool weights = a.logits != nullptr && w.hb == 0;
+  if (!get_work(a, w)) return;
+  // an unsplit sequence is ready but for the weights of kv heads with more than one block of query heads
+  const bool weights = a.logits != nullptr && w.hb == 0 && (w.n > 1 || a.G > 16);
   if (w.len <= 0 || (w.n == 1 && !weights)) return;
   const int tid = threadIdx.x;
-  const int hbs = (a.G + 15) >> 4;
-  const float up = a.dtype == kF16 ? 12.f : 0.f;
-  // log2 of the sum of exponentials of the heads that this workgroup needs, 16 threads to a head
-  const int heads = weights ? a.G : min(16, a.G - 16 * w.hb);
-  for (int g0 = 0; g0 < heads; g0 += 16) {
-    const int g = g0 + (tid >> 4);
-    const float* ml = a.part_ml + ((long)(w.first + (weights ? g >> 4 : 0)) * 16 + (g & 15)) * 2;
-    const long next = (long)w.step * 32;
-    float m = -INFINITY, l = 0.f;
-    if (g < heads)
-      for (int i = tid & 15; i < w.n; i += 16) {
-        const float mi = ml[i * next], li = ml[i * next + 1];
-        const float top = fmaxf(m, mi), mu = top == -INFINITY ? 0.f : top;
-        l = l * pow2(m - mu) + li * pow2(mi - mu);
-        m = top;
-      }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-      const float mi = __shfl_xor(m, o, 64), li = __shfl_xor(l, o, 64);
-      const float top = fmaxf(m, mi), mu = top == -INFINITY ? 0.f : top;
-      l = l * pow2(m - mu) + li * pow2(mi - mu);
-      m = top;
-    }
-    if (g < heads && (tid & 15) == 0) lse[g] = m + log2f(l);
-  }
-  __syncthreads();
   if (w.n > 1) {
-    const int gb = min(16, a.G - 16 * w.hb), E = gb * a.D;
-    int per = ((E + w.n - 1) / w.n + 15) & ~15;
+    const int E = min(16, a.G - 16 * w.hb) * a.D;
+    const int per = ((E + w.n - 1) / w.n + 15) & ~15;
     const int e0 = w.chunk * per, e1 = min(E, e0 + per);
     int wide = 16;
-    while (wide < per && wide < 256) wide *= 2;
-    const int ways = 256 / wide, who = tid / wide;
+    while (wide < per && wide < kJoinThreads) wide *= 2;
+    const int ways = kJoinThreads / wide, who = tid / wide;
     const float* po = a.part_o + (long)w.first * a.gs * a.D;
     const float* ml = a.part_ml + (long)w.first * 32;
-    const long step_o = (long)w.step * a.gs * a.D, step_m = (long)w.step * 32;
+    const long step_o = (long)a.step.d * a.gs * a.D, step_m = (long)a.step.d * 32;
     const long out0 = ((long)w.b * a.H * a.G + w.hk * a.G + 16 * w.hb) * a.D;
     for (int e = e0; e < e1; e += wide) {
       const int at = e + (tid & (wide - 1));
-      float sum = 0.f;
+      float m = -INFINITY, l = 0.f, x = 0.f;
       if (at < e1) {
         const int g = at / a.D;
-        const float ref = lse[g];
-        for (int i = who; i < w.n; i += ways) sum += po[i * step_o + at] * pow2(ml[i * step_m + g * 2] - ref);
+#pragma unroll 4
+        for (int i = who; i < w.n; i += ways)
+          merge(m, l, x, ml[i * step_m + g * 2], ml[i * step_m + g * 2 + 1], po[i * step_o + at]);
       }
-      part[tid] = sum;
+      sm[tid] = m, sl[tid] = l, sx[tid] = x;
       __syncthreads();
       if (who == 0 && at < e1) {
-        for (int i = 1; i < ways; ++i) sum += part[i * wide + tid];
-        store_any(a.dtype, a.o, out0 + at, sum);
+        for (int i = 1; i < ways; ++i) merge(m, l, x, sm[i * wide + tid], sl[i * wide + tid], sx[i * wide + tid]);
+        store_any(a.dtype, a.o, out0 + at, x / l);
       }
       __syncthreads();
     }
   }
   if (weights) {
-    const int* table = a.table + (long)w.b * a.table_b;
-    const float* logit = a.logits + ((long)w.b * a.H + w.hk) * a.cap * a.G;
-    for (int s = w.s0 + tid; s < w.s1; s += 256) {
-      const int p = table[fdiv(s, a.page)];
-      if ((unsigned)p >= (unsigned)a.pages) continue;
-      const long off = s - fdiv(s, a.page) * a.page.d;
-      float sum = 0.f;
-      for (int g = 0; g < a.G; ++g) sum += pow2(logit[(long)s * a.G + g] * a.c - lse[g] + up);
-      a.scores_out[p * a.sos.page + w.hk * a.sos.head + off * a.sos.row] =
-          a.scores[p * a.ss.page + w.hk * a.ss.head + off * a.ss.row] + sum;
+    // log2 of the sum of exponentials of all heads, 16 threads to a head
+    for (int g0 = 0; g0 < a.G; g0 += kJoinThreads / 16) {
+      const int g = g0 + (tid >> 4);
+      const float* ml = a.part_ml + ((long)(w.first + (g >> 4)) * 16 + (g & 15)) * 2;
+      float m = -INFINITY, l = 0.f, x = 0.f;
+      if (g < a.G) {
+#pragma unroll 4
+        for (int i = tid & 15; i < w.n; i += 16) merge(m, l, x, ml[i * (long)a.step.d * 32], ml[i * (long)a.step.d * 32 + 1], 0.f);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) merge(m, l, x, __shfl_xor(m, o, 64), __shfl_xor(l, o, 64), 0.f);
+      if (g < a.G && (tid & 15) == 0) lse[g] = m + log2f(l) - (a.dtype == kF16 ? 12.f : 0.f);
     }
+    __syncthreads();
+    gather_weights(a, w.b, w.hk, w.s0, w.s1, lse);
   }
 }
 
@@ -561,126 +662,294 @@ ZOO_DEV uint32_t rank_key(float score, bool late) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kEvictThreads = 1024;
 constexpr int kEvictBins = 2048;
+constexpr int kEvictHeld = 32768;   // keys that LDS holds
+constexpr int kEvictSeg = 4096;     // slots of a workgroup where a row is shared out
 
-// exclusive prefix sum over the workgroup in thread order; total for everybody. Two barriers.
-ZOO_DEV int block_prefix(int x, int* tmp, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  int upto = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(upto, o, 64);
-    if (lane >= o) upto += y;
-  }
+// exclusive prefix sum over the workgroup in thread order. Two barriers.
+template <int NT>
+ZOO_DEV int block_prefix(int x, int* tmp) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int upto = wave_prefix(x);
   if (lane == 63) tmp[wave] = upto;
   __syncthreads();
   int before = 0;
-  total = 0;
-  for (int i = 0; i < waves; ++i) {
-    const int t = tmp[i];
-    before += i < wave ? t : 0;
-    total += t;
-  }
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) before += i < wave ? tmp[i] : 0;
   __syncthreads();
   return before + upto - x;
 }
 
-// One workgroup per (sequence, kv head): a radix selection of the budget-th largest key (11 + 11 + 10
-// bits, histograms in LDS, the keys too as far as they fit), then one ordered pass that lists the slots
-// given up below the budget and the kept ones behind it, which will take their places.
-__global__ __launch_bounds__(kEvictThreads) void paged_evict_select_kernel(const PagedEvictArgs a, int held) {
-  extern __shared__ uint32_t sh[];  // [held] keys
-  __shared__ int hist[kEvictBins];
-  __shared__ int tmp[kEvictThreads / 64];
-  __shared__ int s_bin, s_left, s_bad;
-  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, tid = threadIdx.x;
-  const int len = seq_len(a.len, b, a.cap);
-  const int* table = a.table + (long)b * a.table_b;
-  if (tid == 0) s_bad = len < 0;
-  __syncthreads();
-  if (len > 0) {
-    bool bad = false;
-    for (int i = tid; i <= (int)fdiv(len - 1, a.page); i += kEvictThreads) bad |= (unsigned)table[i] >= (unsigned)a.pages;
-    if (bad) s_bad = 1;
+// The cut between kept and evicted: a slot is kept if its key is above `key`, or if it equals it and it is among
+// the first `ties` of those.
+struct Cut {
+  uint32_t key;
+  int ties;
+};
+
+// One digit of a radix selection: finds the bin, from the top, that holds the `left`-th largest of the keys counted
+// in `hist`, puts it into the key at `shift` and takes those above it off `left`. True if the bin is kept whole, and
+// the selection is finished: then everything from the bin's lowest key on is kept.
+template <int NT>
+ZOO_DEV bool pick_bin(const int* hist, int shift, uint32_t& key, int& left, int* tmp, int* res) {
+  constexpr int PER = kEvictBins / NT;
+  int n[PER], sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sum += n[i] = hist[kEvictBins - 1 - (int)threadIdx.x * PER - i];
+  int before = block_prefix<NT>(sum, tmp);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (before < left && before + n[i] >= left) {
+      res[0] = kEvictBins - 1 - (int)threadIdx.x * PER - i;
+      res[1] = left - before;
+      res[2] = n[i];
+    }
+    before += n[i];
   }
   __syncthreads();
-  const bool bad = s_bad;
+  key |= (uint32_t)res[0] << shift;
+  left = res[1];
+  const bool whole = res[1] == res[2];
+  __syncthreads();
+  return whole;
+}
+// with every slot of the bin kept, the cut lies below its lowest key (which is not 0: then all would be kept)
+ZOO_DEV Cut cut_of(uint32_t key, int left, bool whole) { return whole ? Cut{key - 1u, 0} : Cut{key, left}; }
+
+constexpr int kShift[3] = {21, 10, 0};
+constexpr uint32_t kAbove[3] = {0u, 0xffe00000u, 0xfffffc00u};   // the digits already known
+constexpr uint32_t kDigit[3] = {2047u, 2047u, 1023u};
+
+// where slot s of a row lies
+struct Row {
+  const int* table;
+  FastDiv page;
+  int h;
+  ZOO_DEV long at(int s, int p, const PoolStride& st) const {
+    return p * st.page + h * st.head + (long)(s - (int)(fdiv(s, page) * page.d)) * st.row;
+  }
+  ZOO_DEV int id(int s) const { return table[fdiv(s, page)]; }
+};
+
+// counts of a stretch of slots: key above the cut or equal to it, below the budget or behind it
+struct Counts {
+  int gt_lo, eq_lo, gt_hi, eq_hi;
+};
+
+template <class Key>
+ZOO_DEV Counts count_range(int s0, int s1, int K, const Cut& cut, Key key) {
+  Counts c{0, 0, 0, 0};
+  for (int s = s0; s < s1; s += 64) {
+    const int at = s + (threadIdx.x & 63);
+    const bool in = at < s1;
+    const uint32_t k = in ? key(at) : 0u;
+    const unsigned long long gt = __ballot(in && k > cut.key), eq = __ballot(in && k == cut.key);
+    const unsigned long long lo = __ballot(at < K);
+    c.gt_lo += __popcll(gt & lo), c.gt_hi += __popcll(gt & ~lo);
+    c.eq_lo += __popcll(eq & lo), c.eq_hi += __popcll(eq & ~lo);
+  }
+  return c;
+}
+
+// Lists, for the slots s0 .. s1 of one wave, those given up below the budget and those kept behind it, in
+// order. `b`: the counts of all slots before s0; `eq_lo`: of the whole row.
+template <class Key>
+ZOO_DEV void list_range(const PagedEvictArgs& a, const Row& row, int s0, int s1, const Counts& b, int eq_lo,
+                        const Cut& cut, int* give, int* take, Key key) {
+  const int lane = threadIdx.x & 63, K = a.budget;
+  const unsigned long long below = (1ull << lane) - 1;
+  const bool copy = a.scores_out != a.scores || a.positions_out != a.positions;
+  int equal = b.eq_lo + b.eq_hi;
+  int gave = min(s0, K) - b.gt_lo - min(cut.ties, b.eq_lo);
+  int took = b.gt_hi + min(max(cut.ties - eq_lo, 0), b.eq_hi);
+  for (int s = s0; s < s1; s += 64) {
+    const int at = s + lane;
+    const bool in = at < s1;
+    const uint32_t k = in ? key(at) : 0u;
+    const unsigned long long eq = __ballot(in && k == cut.key);
+    const bool kept = in && (k > cut.key || (k == cut.key && equal + __popcll(eq & below) < cut.ties));
+    equal += __popcll(eq);
+    const unsigned long long holes = __ballot(in && !kept && at < K), tails = __ballot(kept && at >= K);
+    if (in && !kept && at < K) give[gave + __popcll(holes & below)] = at;
+    if (kept && at >= K) take[took + __popcll(tails & below)] = at;
+    gave += __popcll(holes);
+    took += __popcll(tails);
+    if (copy && kept && at < K) {
+      const int p = row.id(at);
+      a.scores_out[row.at(at, p, a.sos)] = a.scores[row.at(at, p, a.ss)];
+      a.positions_out[row.at(at, p, a.pos)] = a.positions[row.at(at, p, a.ps)];
+    }
+  }
+}
+
+ZOO_DEV uint32_t load_key(const PagedEvictArgs& a, const Row& row, int s, long oldest, bool& bad) {
+  const int p = row.id(s);
+  if ((unsigned)p >= (unsigned)a.pages) {
+    bad = true;
+    return 0u;
+  }
+  return rank_key(a.scores[row.at(s, p, a.ss)], a.positions[row.at(s, p, a.ps)] >= oldest);
+}
+
+// One workgroup per row (sequence and kv head), its keys in LDS: a radix selection of the budget-th largest by
+// digits of 11, 11 and 10 bits, then the lists, each wave a stretch of the slots. Bound by its
+// barriers and the latency of its loads.
+template <int NT>
+__global__ __launch_bounds__(NT) void paged_evict_select_kernel(const PagedEvictArgs a) {
+  extern __shared__ uint32_t keys[];
+  __shared__ int hist[kEvictBins];
+  __shared__ int tmp[NT / 64], res[3], s_bad;
+  __shared__ Counts counts[NT / 64];
+  const int b = blockIdx.x / a.H, tid = threadIdx.x, wave = uni(tid >> 6);
+  const Row row{a.table + (long)b * a.table_b, a.page, (int)blockIdx.x - b * a.H};
+  const int len = seq_len(a.len, b, a.cap), K = a.budget;
+  const long oldest = (long)a.seen[b] - a.recent;
+  if (tid == 0) s_bad = len < 0;
+  for (int i = tid; i < kEvictBins; i += NT) hist[i] = 0;
+  __syncthreads();
+  bool bad = false;
+#pragma unroll 4
+  for (int s = tid; s < len; s += NT) {
+    const uint32_t k = load_key(a, row, s, oldest, bad);
+    keys[s] = k;
+    atomicAdd(&hist[k >> kShift[0]], 1);
+  }
+  if (bad) s_bad = 1;
+  __syncthreads();
+  const bool leave = s_bad;
   if (tid == 0) {
     a.count[blockIdx.x] = 0;
-    // every kv head writes the same number only if no page is bad, and that is the sequence's matter
-    if (h == 0) a.len_out[b] = bad ? a.len[b] : min(len, a.budget);
+    if (row.h == 0) a.len_out[b] = leave ? a.len[b] : min(len, K);
   }
-  if (bad || len == 0) return;
-  auto at = [&](int s, const PoolStride& st) {
-    const int pi = fdiv(s, a.page);
-    return table[pi] * st.page + h * st.head + (long)(s - pi * (int)a.page.d) * st.row;
-  };
-  const long oldest = (long)a.seen[b] - a.recent;
-  auto key_of = [&](int s) { return rank_key(a.scores[at(s, a.ss)], a.positions[at(s, a.ps)] >= oldest); };
-  const int K = a.budget;
-  uint32_t cut = 0;
-  int ties = len;  // keys equal to `cut` that are kept, lowest slots first
+  if (leave || len == 0) return;
+  auto key = [&](int s) { return keys[s]; };
+  Cut cut{0u, len};   // no longer than the budget: all are kept
   if (len > K) {
-    uint32_t prefix = 0;
+    uint32_t known = 0;
     int left = K;
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-      const uint32_t mask = pass == 2 ? 1023u : 2047u;
-      const uint32_t above = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-      for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[i] = 0;
+    bool whole = pick_bin<NT>(hist, kShift[0], known, left, tmp, res);
+    for (int pass = 1; pass < 3 && !whole; ++pass) {
+      for (int i = tid; i < kEvictBins; i += NT) hist[i] = 0;
       __syncthreads();
-      for (int s = tid; s < len; s += kEvictThreads) {
-        uint32_t k;
-        if (pass == 0 || s >= held) {
-          k = key_of(s);
-          if (s < held) sh[s] = k;
-        } else {
-          k = sh[s];
-        }
-        if ((k & above) == prefix) atomicAdd(&hist[(k >> shift) & mask], 1);
-      }
+      for (int s = tid; s < len; s += NT)
+        if ((keys[s] & kAbove[pass]) == known) atomicAdd(&hist[(keys[s] >> kShift[pass]) & kDigit[pass]], 1);
       __syncthreads();
-      // bins from the top: thread t owns bins 2047 - 2t and 2046 - 2t
-      const int b0 = hist[kEvictBins - 1 - 2 * tid], b1 = hist[kEvictBins - 2 - 2 * tid];
-      int total;
-      const int before = block_prefix(b0 + b1, tmp, total);
-      if (before < left && before + b0 >= left) s_bin = kEvictBins - 1 - 2 * tid, s_left = left - before;
-      if (before + b0 < left && before + b0 + b1 >= left) s_bin = kEvictBins - 2 - 2 * tid, s_left = left - before - b0;
-      __syncthreads();
-      prefix |= (uint32_t)s_bin << shift;
-      left = s_left;
-      __syncthreads();
+      whole = pick_bin<NT>(hist, kShift[pass], known, left, tmp, res);
     }
-    cut = prefix;
-    ties = left;
+    cut = cut_of(known, left, whole);
+  }
+  const int per = ((len + NT - 1) / NT) * 64, s0 = min(len, wave * per), s1 = min(len, s0 + per);
+  const Counts mine = count_range(s0, s1, K, cut, key);
+  if ((tid & 63) == 0) counts[wave] = mine;
+  __syncthreads();
+  Counts before{0, 0, 0, 0};
+  int eq_lo = 0;
+  for (int i = 0; i < NT / 64; ++i) {
+    const Counts c = counts[i];
+    eq_lo += c.eq_lo;
+    if (i < wave) before.gt_lo += c.gt_lo, before.eq_lo += c.eq_lo, before.gt_hi += c.gt_hi, before.eq_hi += c.eq_hi;
   }
   int* give = a.moves + (long)blockIdx.x * 2 * a.most;
-  int* take = give + a.most;
-  const bool copy = a.scores_out != a.scores || a.positions_out != a.positions;
-  int equal = 0, gave = 0, took = 0;
-  for (int s0 = 0; s0 < len; s0 += kEvictThreads) {
-    const int s = s0 + tid;
-    const bool in = s < len;
-    const uint32_t k = len <= K ? 0xffffffffu : !in ? 0u : s < held ? sh[s] : key_of(s);
-    int n;
-    const bool eq = in && k == cut;
-    const int nth = equal + block_prefix(eq, tmp, n);
-    equal += n;
-    const bool kept = in && (k > cut || (eq && nth < ties));
-    // gives in the low half, takes in the high half of one sum
-    const bool hole = in && s < K && !kept, tail = kept && s >= K;
-    const int rank = block_prefix((int)hole | ((int)tail << 16), tmp, n);
-    if (hole) give[gave + (rank & 0xffff)] = s;
-    if (tail) take[took + (rank >> 16)] = s;
-    gave += n & 0xffff;
-    took += n >> 16;
-    if (copy && kept && s < K) {
-      a.scores_out[at(s, a.sos)] = a.scores[at(s, a.ss)];
-      a.positions_out[at(s, a.pos)] = a.positions[at(s, a.ps)];
+  list_range(a, row, s0, s1, before, eq_lo, cut, give, give + a.most, key);
+  if (tid == 0) {
+    int gt = 0, eq = 0;   // as many are kept behind the budget as are given up below it
+    for (int i = 0; i < NT / 64; ++i) gt += counts[i].gt_hi, eq += counts[i].eq_hi;
+    a.count[blockIdx.x] = gt + min(max(cut.ties - eq_lo, 0), eq);
+  }
+}
+
+// Rows of more slots than one workgroup should take: the same selection with a row shared out in segments of
+// kEvictSeg, a launch for each step that needs all of the row before it. Histograms of a row add
+// up in memory (whole numbers, so in any order). STEP 0 .. 2: the digits, 3: counts of each wave's stretch, 4: the lists.
+template <int STEP>
+__global__ __launch_bounds__(256) void paged_evict_long_kernel(const PagedEvictArgs a) {
+  __shared__ int hist[kEvictBins];
+  __shared__ int tmp[4], res[3];
+  const int r = blockIdx.x / a.segs, seg = blockIdx.x - r * a.segs, b = r / a.H, tid = threadIdx.x;
+  const Row row{a.table + (long)b * a.table_b, a.page, r - b * a.H};
+  const int len = seq_len(a.len, b, a.cap), K = a.budget;
+  int* flag = a.hist + (long)r * kEvictRow;     // a page of the row is bad
+  int* state = flag + 1;                        // [3][3] known bits, left, whole, after each digit
+  int* sums = flag + 16;                        // [3][kEvictBins]
+  if (STEP == 0 && seg == 0 && tid == 0) a.count[r] = 0;
+  if (STEP > 0 && seg == 0 && tid == 0 && STEP == 4 && row.h == 0) a.len_out[b] = len < 0 || *flag ? a.len[b] : min(len, K);
+  const int s0 = seg * kEvictSeg, s1 = min(len, s0 + kEvictSeg);
+  if (s0 >= s1) return;
+  uint32_t* keys = (uint32_t*)a.keys + (long)r * a.cap;
+  if constexpr (STEP == 0) {
+    const long oldest = (long)a.seen[b] - a.recent;
+    for (int i = tid; i < kEvictBins; i += 256) hist[i] = 0;
+    __syncthreads();
+    bool bad = false;
+#pragma unroll 4
+    for (int s = s0 + tid; s < s1; s += 256) {
+      const uint32_t k = load_key(a, row, s, oldest, bad);
+      keys[s] = k;
+      atomicAdd(&hist[k >> kShift[0]], 1);
+    }
+    if (bad) atomicOr(flag, 1);
+  } else {
+    if (*flag) return;
+    uint32_t known = 0;
+    int left = K;
+    bool whole = false;
+    if (len > K) {
+      if (STEP > 1) {
+        const int* st = state + 3 * (min(STEP, 4) - 2);
+        known = st[0], left = st[1], whole = st[2];
+      }
+      if (STEP <= 3 && !whole) {
+        // the histogram that the step before filled
+        constexpr int d = STEP <= 3 ? STEP - 1 : 0;
+        for (int i = tid; i < kEvictBins; i += 256) hist[i] = sums[d * kEvictBins + i];
+        __syncthreads();
+        whole = pick_bin<256>(hist, kShift[d], known, left, tmp, res);
+      }
+      if (STEP <= 3 && seg == 0 && tid == 0) {
+        int* st = state + 3 * (STEP - 1);
+        st[0] = known, st[1] = left, st[2] = whole;
+      }
+    }
+    if constexpr (STEP <= 2) {
+      if (len <= K || whole) return;
+      for (int i = tid; i < kEvictBins; i += 256) hist[i] = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (int s = s0 + tid; s < s1; s += 256) {
+        const uint32_t k = keys[s];
+        if ((k & kAbove[STEP]) == known) atomicAdd(&hist[(k >> kShift[STEP]) & kDigit[STEP]], 1);
+      }
+    } else {
+      const Cut cut = len > K ? cut_of(known, left, whole) : Cut{0u, len};
+      const int wave = uni(tid >> 6), w0 = min(s1, s0 + wave * (kEvictSeg / 4)), w1 = min(s1, w0 + kEvictSeg / 4);
+      auto key = [&](int s) { return keys[s]; };
+      Counts* counts = (Counts*)(a.hist + (long)a.B * a.H * kEvictRow) + (long)r * a.segs * 4;
+      if constexpr (STEP == 3) {
+        const Counts c = count_range(w0, w1, K, cut, key);
+        if ((tid & 63) == 0) counts[seg * 4 + wave] = c;
+      } else {
+        // the stretches before this wave's, and those of the whole row, a few to each lane
+        const int used = ((len - 1) / kEvictSeg + 1) * 4, here = seg * 4 + wave;
+        Counts before{0, 0, 0, 0}, all{0, 0, 0, 0};
+        for (int i = tid & 63; i < used; i += 64) {
+          const Counts c = counts[i];
+          all.eq_lo += c.eq_lo, all.gt_hi += c.gt_hi, all.eq_hi += c.eq_hi;
+          if (i < here) before.gt_lo += c.gt_lo, before.eq_lo += c.eq_lo, before.gt_hi += c.gt_hi, before.eq_hi += c.eq_hi;
+        }
+        auto sum = [](int x) { return __builtin_amdgcn_readlane(wave_prefix(x), 63); };
+        before = {sum(before.gt_lo), sum(before.eq_lo), sum(before.gt_hi), sum(before.eq_hi)};
+        const int eq_lo = sum(all.eq_lo), gt_hi = sum(all.gt_hi), eq_hi = sum(all.eq_hi);
+        int* give = a.moves + (long)r * 2 * a.most;
+        list_range(a, row, w0, w1, before, eq_lo, cut, give, give + a.most, key);
+        if (seg == 0 && tid == 0) a.count[r] = gt_hi + min(max(cut.ties - eq_lo, 0), eq_hi);
+      }
     }
   }
-  if (tid == 0) a.count[blockIdx.x] = gave;
+  if constexpr (STEP <= 2) {
+    __syncthreads();
+    for (int i = tid; i < kEvictBins; i += 256)
+      if (hist[i] != 0) atomicAdd(&sums[STEP * kEvictBins + i], hist[i]);
+  }
 }
 
 // moves what the lists say: 256 / vec rows at a time
@@ -718,8 +987,8 @@ hipError_t attn_launch(const PagedAttnArgs& a, int items, hipStream_t st) {
   }
   paged_attn_kernel<DT, DP, PAD, P16><<<items, 256, lds, st>>>(a);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && (!a.single || a.logits != nullptr)) {
-    paged_attn_join_kernel<<<items, 256, 0, st>>>(a, Tile<DT, DP>::GRAIN);
+  if (e == hipSuccess && (!a.single || (a.logits != nullptr && a.G > 16))) {
+    paged_attn_join_kernel<<<items, kJoinThreads, 0, st>>>(a);
     e = hipGetLastError();
   }
   return e;
@@ -754,18 +1023,36 @@ extern "C" hipError_t zoo_paged_append(const zoo::PagedAppendArgs* a, hipStream_
   return hipGetLastError();
 }
 
+extern "C" long zoo_paged_evict_scratch(const zoo::PagedEvictArgs* a) {
+  return a->segs > 0 ? (long)a->B * a->H * (zoo::kEvictRow + a->segs * 16) : 0;
+}
+
 extern "C" hipError_t zoo_paged_evict(const zoo::PagedEvictArgs* a, hipStream_t st) {
-  const int held = a->cap < 32768 ? a->cap : 32768;
-  const size_t lds = (size_t)held * 4;
-  if (lds > 32768) {
-    const hipError_t e = hipFuncSetAttribute((const void*)zoo::paged_evict_select_kernel,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
+  const int rows = a->B * a->H;
+  hipError_t e;
+  if (a->segs > 0) {
+    const unsigned grid = (unsigned)rows * a->segs;
+    zoo::paged_evict_long_kernel<0><<<grid, 256, 0, st>>>(*a);
+    zoo::paged_evict_long_kernel<1><<<grid, 256, 0, st>>>(*a);
+    zoo::paged_evict_long_kernel<2><<<grid, 256, 0, st>>>(*a);
+    zoo::paged_evict_long_kernel<3><<<grid, 256, 0, st>>>(*a);
+    zoo::paged_evict_long_kernel<4><<<grid, 256, 0, st>>>(*a);
+  } else {
+    const size_t lds = (size_t)(a->cap > 0 ? a->cap : 1) * 4;
+    if (a->cap <= 2048) {
+      zoo::paged_evict_select_kernel<256><<<rows, 256, lds, st>>>(*a);
+    } else {
+      if (lds > 32768) {
+        e = hipFuncSetAttribute((const void*)zoo::paged_evict_select_kernel<1024>,
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+      }
+      zoo::paged_evict_select_kernel<1024><<<rows, 1024, lds, st>>>(*a);
+    }
   }
-  zoo::paged_evict_select_kernel<<<a->B * a->H, zoo::kEvictThreads, lds, st>>>(*a, held);
-  hipError_t e = hipGetLastError();
+  e = hipGetLastError();
   if (e != hipSuccess || a->most <= 0) return e;
   const long per = ((long)a->most * a->vec.d + 255) / 256;
-  zoo::paged_evict_move_kernel<<<(unsigned)(per * a->B * a->H), 256, 0, st>>>(*a, (int)per);
+  zoo::paged_evict_move_kernel<<<(unsigned)(per * rows), 256, 0, st>>>(*a, (int)per);
   return hipGetLastError();
 }

@@ -204,6 +204,7 @@ hipError_t zoo_attn_bwd(const void*, const void*, const void*, const void*, cons
                         hipStream_t);
 hipError_t zoo_paged_attn(const zoo::PagedAttnArgs*, int, hipStream_t);
 hipError_t zoo_paged_append(const zoo::PagedAppendArgs*, hipStream_t);
+long zoo_paged_evict_scratch(const zoo::PagedEvictArgs*);
 hipError_t zoo_paged_evict(const zoo::PagedEvictArgs*, hipStream_t);
 }
 
@@ -3205,18 +3206,23 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   auto o = torch::empty({c.B, c.H * G, c.D}, q.options());
   if (o.numel() == 0) return o;
   const int64_t per_seq = c.H * hbs;
-  // chunks to aim at: enough to fill the chip, and no longer than the mean sequence, so that one long
-  // sequence among short ones is shared out
+  // Chunks to aim at: what the chip runs at once (two workgroups to a CU, one of the 256-wide kernels), but no
+  // fewer than there are sequences, so that a long one among short ones is shared out.
   static const int64_t cus = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int64_t target = std::max<int64_t>(c.B, (3 * cus + per_seq - 1) / per_seq);
+  const int64_t at_once = (c.D > 128 ? 1 : 2) * cus / per_seq;
+  const int64_t target = std::max<int64_t>({c.B, at_once, 1});
   zoo::PagedAttnArgs a{};
-  a.single = c.cap <= 256;
-  const int64_t items = (a.single ? c.B : c.B + target) * per_seq;
+  a.single = c.cap * c.D * c.es * 2 <= 256 * 1024;
+  const int64_t items = (a.single ? c.B : c.B + target + target / 512 + 1) * per_seq;
   TORCH_CHECK(items < (1LL << 31), what, ": too many heads in the batch");
   auto f32 = q.options().dtype(at::kFloat);
-  torch::Tensor ml, po, logits;
+  torch::Tensor ml, po, logits, plan;
   const int64_t gs = std::min<int64_t>(G, 16);
-  if (!a.single || weights) ml = torch::empty({items, 16, 2}, f32);
+  if (!a.single || (weights && G > 16)) {
+    ml = torch::empty({items, 16, 2}, f32);
+    plan = torch::empty({items, 8}, lengths.options());
+    a.plan = reinterpret_cast<int4*>(plan.data_ptr<int>());
+  }
   if (!a.single) po = torch::empty({items, gs, c.D}, f32);
   if (weights) logits = torch::empty({c.B, c.H, c.cap, G}, f32);
   a.q = q.data_ptr(), a.k = kp.data_ptr(), a.v = vp.data_ptr();
@@ -3233,7 +3239,8 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   a.ks = pool_stride(kp), a.vs = pool_stride(vp);
   a.page = fast_div((uint32_t)c.page);
   a.B = c.B, a.H = c.H, a.G = G, a.D = c.D, a.pages = c.P, a.cap = c.cap, a.dtype = c.dtype, a.gs = gs;
-  a.target = target;
+  a.hbs = hbs, a.step = fast_div((uint32_t)per_seq);
+  a.per_target = (float)(0.999 / target), a.at_once = at_once >= c.B ? at_once : 0;
   a.c = (float)(scale * 1.4426950408889634);
   check_hip(zoo_paged_attn(&a, (int)items, cur_stream()), what);
   return o;
@@ -3321,6 +3328,14 @@ torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scor
   a.page = fast_div((uint32_t)c.page), a.vec = fast_div((uint32_t)vec);
   a.B = c.B, a.H = c.H, a.pages = c.P, a.cap = c.cap, a.es = c.es;
   a.budget = budget, a.recent = recent, a.most = most;
+  a.segs = c.cap > 16384 ? (c.cap + 4095) / 4096 : 0;
+  TORCH_CHECK(rows * std::max(a.segs, 1) < (1LL << 31), what, ": too many heads or slots in the batch");
+  torch::Tensor hist, keys;
+  if (a.segs > 0) {
+    hist = torch::zeros({(int64_t)zoo_paged_evict_scratch(&a)}, lengths.options());
+    keys = torch::empty({rows * c.cap}, lengths.options());
+    a.hist = hist.data_ptr<int>(), a.keys = keys.data_ptr<int>();
+  }
   check_hip(zoo_paged_evict(&a, cur_stream()), what);
   return len_out;
 }

@@ -313,6 +313,20 @@ def evict_by_definition(pools, table, lengths, seen, budget, recent):
     return k, v, scores, positions
 
 
+EVICT_LONG = [      # rows shared out over workgroups
+    (1, 8, 64, FL, "phsd", [40000, 17, 9000], 6000, 100, "ties"),
+    (2, 8, 100, BF, "pshd", [20000, 8193, 4096, 0], 4096, 0, "plain"),
+    (1, 16, 128, BF, "phsd", [17000], 16999, 16999, "odd"),
+    (1, 8, 7, FL, "phsd", [30000, 12345], 12345, 77, "zeros"),
+]
+
+
+@GPU
+@pytest.mark.parametrize("H,D,page,dtype,order,lengths,budget,recent,kind", EVICT_LONG)
+def test_evict_long(gpu, H, D, page, dtype, order, lengths, budget, recent, kind):
+    test_evict("cuda", H, D, page, dtype, order, lengths, budget, recent, kind)
+
+
 @pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
 @pytest.mark.parametrize("H,D,page,dtype,order,lengths,budget,recent,kind", [
     (2, 64, 16, BF, "phsd", [100, 0, 50, 51, 1], 50, 10, "plain"),
