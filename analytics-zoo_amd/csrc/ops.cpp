@@ -212,6 +212,9 @@ namespace {
 
 hipStream_t cur_stream() { return at::hip::getCurrentHIPStream().stream(); }
 
+// the error a runtime call left behind, which the next launch's check would report otherwise; cleared
+int take_last_error() { return (int)hipGetLastError(); }
+
 void check_hip(hipError_t e, const char* what) {
   TORCH_CHECK(e == hipSuccess, "zoo HIP kernel launch failed in ", what, ": ", hipGetErrorString(e));
 }
@@ -3806,6 +3809,7 @@ PYBIND11_MODULE(_C, m) {
   m.def("attn_bwd", &attn_bwd, py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("mask"),
         py::arg("o"), py::arg("lse"), py::arg("causal"), py::arg("pdrop") = 0.0, py::arg("seed") = 0);
   m.def("attn_bwd_strided", &attn_bwd_strided);
+  m.def("take_last_error", &take_last_error);
   m.def("paged_attention", &paged_attention);
   m.def("paged_append", &paged_append);
   m.def("paged_evict", &paged_evict);

@@ -7,7 +7,8 @@ the JVM (``Zs/serving/ClusterServing.scala:192-203`` PreProcessing), which has n
 such lock. Here the decode runs in a pool of spawned helper processes (numpy +
 PIL only, they never touch the GPU) that write RGB pixels straight into a ring of
 shared-memory batch slots; the worker pins each slot with ``hipHostRegister`` once,
-so a decoded batch goes to HBM with a single async copy.
+so a decoded batch goes to HBM with a single async copy. Where the driver refuses to pin
+memory that exists already, a batch is copied into a pinned tensor of its own first.
 """
 import multiprocessing as mp
 import os
@@ -44,11 +45,15 @@ class ProcDecodePool:
             shm = shared_memory.SharedMemory(create=True, size=int(np.prod(shape)))
             arr = np.ndarray(shape, np.uint8, buffer=shm.buf)
             views = [torch.from_numpy(arr[s]) for s in range(self.nslots)]
+            stage = None
             if torch.cuda.is_available():
                 cudart = torch.cuda.cudart()
                 # page-lock the shared block so H2D copies of a slot are async DMA
-                cudart.cudaHostRegister(arr.ctypes.data, arr.nbytes, 0)
-            r = self.rings[key] = [shm, arr, views, 0, shape]
+                if int(cudart.cudaHostRegister(arr.ctypes.data, arr.nbytes, 0)) != 0:
+                    from zoo.ops._native import native
+                    native().take_last_error()   # or the next kernel launch would report the refusal
+                    stage = [torch.empty(shape[1:], dtype=torch.uint8, pin_memory=True) for _ in views]
+            r = self.rings[key] = [shm, arr, views, 0, shape, stage]
         return r
 
     def decode(self, payloads):
@@ -63,14 +68,14 @@ class ProcDecodePool:
         tasks = [(r[0].name, r[4], slot, o, payloads[o:o + step]) for o in range(0, B, step)]
         if not all(self.pool.starmap(_w.decode_into, tasks)):
             return None
-        return r[2][slot]
+        return r[2][slot] if r[5] is None else r[5][slot].copy_(r[2][slot])
 
     def close(self):
         import torch
         self.pool.terminate()
         for r in self.rings.values():
             shm, arr = r[0], r[1]
-            if torch.cuda.is_available():
+            if torch.cuda.is_available() and r[5] is None:
                 try:
                     torch.cuda.cudart().cudaHostUnregister(arr.ctypes.data)
                 except Exception:  # noqa: BLE001
