@@ -11,4 +11,4 @@ from zoo.ops.pool import max_pool2d_nhwc, global_avg_pool_nhwc
 from zoo.ops.loss import prob_nll, softmax_cross_entropy
 from zoo.ops.nn import layer_norm, embedding, dropout_add, depthwise_conv2d_nhwc, lrn_channels_last
 from zoo.ops.attention import attention
-from zoo.ops.kvcache import paged_append, paged_attention, paged_evict
+from zoo.ops.kvcache import paged_append, paged_attention, paged_evict, PagedKVCache

@@ -8,6 +8,7 @@ says how many slots are in use. Entries of the table behind the last slot in use
     paged_append      writes the keys and values of new tokens behind the slots in use
     paged_attention   attention of one new token per sequence over the slots in use
     paged_evict       cuts sequences down to a budget of slots, by the attention weight each slot gathered
+    PagedKVCache      the pools of all layers of a model and the book of their pages
 
 Eviction needs two more pools ``[pages, kv_heads, page]``: ``scores`` (float32, the attention weight a slot
 has gathered) and ``positions`` (int32, which token a slot holds). Both have a head axis, because after an
@@ -88,6 +89,137 @@ def paged_evict(k_pages, v_pages, scores, positions, page_table, lengths, seen, 
                                     scores_out, positions_out)
     return _evict_ref(k_pages, v_pages, scores, positions, page_table, lengths, seen, budget, recent, scores_out,
                       positions_out)
+
+
+class PagedKVCache:
+    """The caches of all layers of a model that generates for up to ``batch`` sequences at a time, and the host's book
+    of their pages. The layers share one page table: layer ``i`` owns the kv heads ``i * kv_heads ..`` of the pools, so
+    a page holds the same slots of every layer and one ``paged_evict`` serves them all.
+
+    A row's pages are taken as it grows (:meth:`reserve`) and given back by :meth:`release`; ``pages`` bounds their
+    number, by default ``batch`` sequences of ``max_length`` slots. With ``budget``, sequences longer than ``budget +
+    slack`` slots are cut down to ``budget`` after a step; their last ``recent`` tokens stay.
+
+    A step of every layer: :meth:`append`, :meth:`attend` per layer, then :meth:`advance`. Inside a captured hipGraph
+    no page can be taken, so ``reserve`` what the replays will need first, and tell the host's book about them
+    with :meth:`replayed`."""
+
+    def __init__(self, n_layer, batch, max_length, kv_heads, head_dim, page=64, pages=None, budget=None, recent=None,
+                 slack=0, dtype=None, device=None):
+        if min(n_layer, batch, max_length, kv_heads, head_dim, page) < 1:
+            raise ValueError("PagedKVCache: sizes must be at least 1")
+        if budget is not None and budget < 1:
+            raise ValueError("PagedKVCache: budget must be at least 1")
+        if slack < 0 or budget is None and (recent is not None or slack):
+            raise ValueError("PagedKVCache: recent and slack go with a budget, slack not below 0")
+        recent = 0 if recent is None else recent
+        if budget is not None and not 0 <= recent <= budget:
+            raise ValueError("PagedKVCache: recent must be from 0 to the budget")
+        device = torch.device("cuda" if torch.cuda.is_available() else "cpu") if device is None else torch.device(device)
+        dtype = (torch.bfloat16 if device.type == "cuda" else torch.float32) if dtype is None else dtype
+        self.n_layer, self.kv_heads, self.page, self.max_length = n_layer, kv_heads, page, max_length
+        self.budget, self.recent, self.slack = budget, recent, slack
+        width = -(-max_length // page)
+        pages = batch * width if pages is None else pages
+        shape = (pages, n_layer * kv_heads, page)
+        self.k = torch.zeros(*shape, head_dim, dtype=dtype, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.scores = torch.zeros(shape, device=device) if budget is not None else None
+        self.positions = torch.zeros(shape, dtype=torch.int32, device=device) if budget is not None else None
+        self.page_table = torch.full((batch, width), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)   # slots in use
+        self.seen = torch.zeros(batch, dtype=torch.int32, device=device)      # tokens each sequence has had
+        self._free = list(range(pages - 1, -1, -1))
+        self._pages = [[] for _ in range(batch)]
+        self._slots = [0] * batch                                             # the host's copy of lengths
+
+    @property
+    def batch(self):
+        return len(self._slots)
+
+    def layer(self, i):
+        """(k_pages, v_pages, scores, positions) of layer ``i``, views of the pools."""
+        h = slice(i * self.kv_heads, (i + 1) * self.kv_heads)
+        return (self.k[:, h], self.v[:, h], None if self.scores is None else self.scores[:, h],
+                None if self.positions is None else self.positions[:, h])
+
+    def reserve(self, tokens, rows=None):
+        """Takes the pages that ``tokens`` (a number, or one for each row) more tokens of the rows need."""
+        rows = range(self.batch) if rows is None else rows
+        tokens = [tokens] * len(rows) if isinstance(tokens, int) else list(tokens)
+        want = [-(-(self._slots[r] + t) // self.page) for r, t in zip(rows, tokens)]
+        if any(self._slots[r] + t > self.max_length for r, t in zip(rows, tokens)):
+            raise RuntimeError("PagedKVCache: a sequence would be longer than max_length = %d slots" % self.max_length)
+        if sum(max(0, w - len(self._pages[r])) for r, w in zip(rows, want)) > len(self._free):
+            raise RuntimeError("PagedKVCache: no pages left")
+        for r, w in zip(rows, want):
+            n = len(self._pages[r])
+            if w > n:
+                self._pages[r] += [self._free.pop() for _ in range(w - n)]
+                self.page_table[r, n:w] = torch.tensor(self._pages[r][n:], dtype=torch.int32).to(self.page_table.device)
+
+    def release(self, rows=None):
+        """Empties rows and gives their pages back."""
+        for r in range(self.batch) if rows is None else rows:
+            self._free += self._pages[r]
+            self._pages[r], self._slots[r] = [], 0
+            self.page_table[r] = -1
+            self.lengths[r] = 0
+            self.seen[r] = 0
+
+    def append(self, i, k, v, counts=None, rows=None):
+        """``paged_append`` to layer ``i``; returns the new lengths, which :meth:`advance` makes the cache's."""
+        kp, vp, scores, positions = self.layer(i)
+        at = slice(None) if rows is None else rows
+        return paged_append(k, v, kp, vp, self.page_table[at], self.lengths[at], counts=counts, seen=self.seen[at],
+                            scores=scores, positions=positions)
+
+    def attend(self, i, q, lengths, scale=None):
+        """``paged_attention`` over layer ``i`` of all rows, gathering weights if there is a budget."""
+        kp, vp, scores, _ = self.layer(i)
+        return paged_attention(q, kp, vp, self.page_table, lengths, scale=scale, scores=scores)
+
+    def advance(self, tokens, lengths, rows=None, evict=True):
+        """Ends a step that gave the rows ``tokens`` tokens (a number, or one for each row): ``lengths`` are in use now,
+        less what eviction takes."""
+        r = range(self.batch) if rows is None else rows
+        tokens = [tokens] * len(r) if isinstance(tokens, int) else list(tokens)
+        if rows is None:
+            self.seen += lengths - self.lengths
+            self.lengths.copy_(lengths)
+        else:
+            self.seen[rows] += lengths - self.lengths[rows]
+            self.lengths[rows] = lengths
+        for x, t in zip(r, tokens):
+            self._slots[x] += t
+        if evict:
+            self.evict()
+
+    def evict(self):
+        """Cuts the sequences down to the budget if one is longer than budget + slack slots, and gives back the pages
+        that a sequence of budget + slack + 1 slots does not need."""
+        if self.budget is None or max(self._slots) <= self.budget + self.slack:
+            return
+        new = paged_evict(self.k, self.v, self.scores, self.positions, self.page_table, self.lengths, self.seen,
+                          self.budget, self.recent)
+        self.lengths.copy_(new)
+        self._slots = [min(n, self.budget) for n in self._slots]
+        if self.k.is_cuda and torch.cuda.is_current_stream_capturing():
+            return
+        keep = -(-(self.budget + self.slack + 1) // self.page)
+        for r, own in enumerate(self._pages):
+            if len(own) > keep:
+                self._free += own[keep:]
+                del own[keep:]
+                self.page_table[r, keep:] = -1
+
+    def replayed(self, tokens=1, evicts=False):
+        """Tells the host's book that a captured step, which gave every row ``tokens`` tokens and ended with an eviction
+        if ``evicts``, was replayed; the capture itself has been counted, as the first replay."""
+        slots = [min(n + tokens, self.budget) if evicts else n + tokens for n in self._slots]
+        if any(n > len(own) * self.page for n, own in zip(slots, self._pages)):
+            raise RuntimeError("PagedKVCache: the replayed step ran past the pages that were reserved for it")
+        self._slots = slots
 
 
 # ---------------------------------------------------------------------------- PyTorch implementation

@@ -70,9 +70,20 @@ class _Block(nn.Module):
         self.ln2_g, self.ln2_b = nn.Parameter(torch.ones(hidden)), nn.Parameter(torch.zeros(hidden))
         self.hidden_drop, self.attn_drop, self.gelu = hidden_drop, attn_drop, gelu
 
-    def forward(self, x, mask=None, causal=False):
-        B, L, H = x.shape
-        nh, hd = self.n_head, H // self.n_head
+    def _attend(self, qkv, mask, causal):
+        B, L, H3 = qkv.shape
+        nh, hd = self.n_head, H3 // (3 * self.n_head)
+        # strided fused kernels (attention-probability dropout in-kernel), no head copies
+        a = attention_packed(qkv, nh, mask=mask, causal=causal, dropout_p=self.attn_drop, training=self.training)
+        if a is None:
+            qkv = qkv.reshape(B, L, 3, nh, hd).permute(2, 0, 3, 1, 4)  # [3, B, nh, L, hd]
+            a = ops.attention(qkv[0], qkv[1], qkv[2], mask=mask, causal=causal, dropout_p=self.attn_drop,
+                              training=self.training)
+            a = a.transpose(1, 2).reshape(B, L, H3 // 3)
+        return a
+
+    def forward(self, x, mask=None, causal=False, cached=None):
+        """``cached``: attention by way of a key/value cache, a function of the packed projection."""
         # x and n each feed a linear and a residual add: the add's x-gradient is folded into
         # the linear's data-gradient GEMM (GradAdd) instead of a separate autograd sum
         h1, h2 = (GradAdd(), GradAdd()) if _RESID_GRAD_FUSE else (None, None)
@@ -83,13 +94,7 @@ class _Block(nn.Module):
             lx = getattr(x, "_zoo_grad_in", None)
             ln_n, ln_out = GradAdd(), GradAdd()
         qkv = ops.linear(x, self.qkv_w, self.qkv_b, grad_add=h1)     # [B, L, 3H]
-        # strided fused kernels (attention-probability dropout in-kernel), no head copies
-        a = attention_packed(qkv, nh, mask=mask, causal=causal, dropout_p=self.attn_drop, training=self.training)
-        if a is None:
-            qkv = qkv.reshape(B, L, 3, nh, hd).permute(2, 0, 3, 1, 4)  # [3, B, nh, L, hd]
-            a = ops.attention(qkv[0], qkv[1], qkv[2], mask=mask, causal=causal, dropout_p=self.attn_drop,
-                              training=self.training)
-            a = a.transpose(1, 2).reshape(B, L, H)
+        a = self._attend(qkv, mask, causal) if cached is None else cached(qkv)
         a = ops.linear(a, self.proj_w, self.proj_b)
         n = _res_ln(a, x, self.hidden_drop, self.training, self.ln1_g, self.ln1_b, self.ln_eps,
                     h1 if h1 is not None else lx, ln_n)
@@ -158,6 +163,78 @@ class TransformerLayer(Layer):
             outs.append(x)
         pooled = torch.tanh(ops.linear(x[:, 0], self.pool_w, self.pool_b))
         return outs + [pooled] if self.output_all_block else [x, pooled]
+
+    # ---- token by token: the keys and values of what was seen stay in a cache ----
+    def init_cache(self, batch, max_length=None, page=64, pages=None, budget=None, recent=None, slack=0):
+        """A :class:`zoo.ops.PagedKVCache` for up to ``batch`` sequences of ``max_length`` (default: the layer's
+        sequence length) slots. With ``budget`` a sequence keeps that many slots per head, the last ``recent`` tokens
+        and those that gathered the most attention."""
+        max_length = self.seq_len if max_length is None else max_length
+        if max_length is None:
+            raise ValueError("init_cache: max_length is needed for a layer without a sequence length")
+        w = self.blocks[0].qkv_w
+        return ops.PagedKVCache(self.n_block, batch, max_length, self.n_head, self.hidden // self.n_head, page=page,
+                                pages=pages, budget=budget, recent=recent, slack=slack, device=w.device)
+
+    def _cached_run(self, x, cached):
+        if self.bidirectional:
+            raise RuntimeError("a bidirectional TransformerLayer sees the whole sequence: it cannot go token by token")
+        if self.training:
+            raise RuntimeError("generation with a cache needs eval(): dropout would act on it")
+        for i, blk in enumerate(self.blocks):
+            x = blk(x, None, causal=True, cached=lambda qkv, i=i, blk=blk: cached(i, blk, qkv))
+        return x
+
+    @staticmethod
+    def _split(qkv, blk, cache):
+        B, T, H3 = qkv.shape
+        v5 = qkv.to(cache.k.dtype).view(B, T, 3, blk.n_head, H3 // (3 * blk.n_head))
+        return v5[:, :, 0], v5[:, :, 1], v5[:, :, 2]
+
+    @torch.no_grad()
+    def prefill(self, xs, cache, counts=None, rows=None):
+        """The prompts ``xs`` = [token_ids, position_ids] ([n, T]) into ``cache``: as rows ``rows`` (a list of n row
+        numbers), which must be empty, all by default. ``counts`` (a list): how many tokens of each prompt are real,
+        the rest is padding behind them. Returns the sequence output [n, T, hidden], as the layer's own call
+        does."""
+        n, T = xs[0].shape
+        at = list(range(cache.batch)) if rows is None else list(rows)
+        counts = [T] * n if counts is None else [int(c) for c in counts]
+        if len(at) != n or len(counts) != n or len(set(at)) != n:
+            raise ValueError("prefill: a row of the cache and a count for each prompt")
+        if not all(0 <= c <= T for c in counts):
+            raise ValueError("prefill: counts from 0 to the prompts' length")
+        if any(cache._slots[r] for r in at):
+            raise RuntimeError("prefill: the cache's rows are in use: release them first")
+        cache.reserve(counts, at)
+        real = torch.tensor(counts, dtype=torch.int32).to(cache.k.device)
+        sub = None if rows is None else torch.tensor(at).to(cache.k.device)
+        new = []
+
+        def cached(i, blk, qkv):
+            _, k, v = self._split(qkv, blk, cache)
+            new[:] = [cache.append(i, k, v, counts=real, rows=sub)]
+            return blk._attend(qkv, None, True)
+        x = self._cached_run(self._embed(xs), cached)
+        cache.advance(counts, new[0], None if rows is None else at, evict=False)
+        return x
+
+    @torch.no_grad()
+    def decode(self, xs, cache):
+        """One token of every row of ``cache``: ``xs`` = [token_ids, position_ids] ([batch]). Returns the sequence
+        output of these tokens [batch, hidden]."""
+        if xs[0].dim() != 1 or xs[0].shape[0] != cache.batch:
+            raise ValueError("decode: one token for each row of the cache")
+        cache.reserve(1)
+        new = []
+
+        def cached(i, blk, qkv):
+            q, k, v = self._split(qkv, blk, cache)
+            new[:] = [cache.append(i, k, v)]
+            return cache.attend(i, q[:, 0], new[0]).reshape(qkv.shape[0], 1, -1).to(qkv.dtype)
+        x = self._cached_run(self._embed([t.unsqueeze(1) for t in xs]), cached)
+        cache.advance(1, new[0])
+        return x[:, 0]
 
 
 class BERT(Layer):

@@ -1,0 +1,246 @@
+"""Token-by-token running of a causal TransformerLayer over a paged key/value cache: append, attention, eviction and
+the host's book of pages as they are used together."""
+import pytest
+import torch
+
+from zoo.ops import PagedKVCache, paged_append, paged_attention, paged_evict
+from zoo.pipeline.api.keras.layers import TransformerLayer
+
+DEVS = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+VOCAB = 60
+
+
+def layer(dev, hidden=64, heads=4, blocks=2, std=0.3, seq_len=48):
+    torch.manual_seed(3)
+    t = TransformerLayer.init(vocab=VOCAB + 200, seq_len=seq_len, n_block=blocks, hidden_size=hidden, n_head=heads,
+                              initializer_range=std)
+    return t.to(dev).eval()
+
+
+def ids(B, T, dev, first=0):
+    g = torch.Generator().manual_seed(1)
+    tok = torch.randint(0, VOCAB, (B, T), generator=g)
+    pos = (torch.arange(T) + VOCAB + first).expand(B, T)
+    return tok.to(dev), pos.to(dev)
+
+
+def near(a, b, dev, hidden=64, std=0.3):
+    """The outputs of a block's LayerNorm are of size 1. On the CPU both sides are float32. On the GPU either rounds its
+    activations to bfloat16 at about ten places per block, 2^-9 rms each (a uniform error of at most 2^-8), and both
+    do: sqrt(2 * 10 * blocks) 2^-9 = 0.012 of the norm for 2 blocks. The softmax magnifies that: queries and keys
+    have components of size std sqrt(hidden), so logits are of size std^2 hidden (23 for 256 wide and 0.3), a relative
+    error e of queries or keys moves a logit by e std^2 hidden, and the weights by as much relative to themselves: an
+    error of 0.012 (1 + std^2 hidden), with 2 for the estimate's own spread."""
+    a, b = a.float().cpu(), b.float().cpu()
+    tol = 1e-4 if dev == "cpu" else 2 * 0.0124 * (1 + std * std * hidden)
+    assert torch.isfinite(a).all()
+    assert ((a - b).norm() / b.norm()).item() < tol
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("hidden,heads,page,std", [
+    (64, 4, 16, 0.3), (128, 2, 7, 0.3), (256, 2, 64, 0.3), (256, 2, 64, 0.02), (256, 4, 16, 0.02)])
+def test_decoding_equals_the_whole_sequence(dev, hidden, heads, page, std):
+    t = layer(dev, hidden, heads, std=std)
+    tok, pos = ids(3, 40, dev)
+    with torch.no_grad():
+        want = t([tok, pos])[0]
+    cache = t.init_cache(3, page=page)
+    near(t.prefill([tok[:, :25], pos[:, :25]], cache), want[:, :25], dev, hidden, std)
+    for i in range(25, 40):
+        near(t.decode([tok[:, i], pos[:, i]], cache), want[:, i], dev, hidden, std)
+    assert cache.lengths.tolist() == [40] * 3 and cache.seen.tolist() == [40] * 3
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_padded_prompts_and_rows_that_come_and_go(dev):
+    t = layer(dev)
+    tok, pos = ids(4, 30, dev)
+    counts = [30, 1, 17, 0]
+    with torch.no_grad():
+        want = t([tok, pos])[0]
+    cache = t.init_cache(4, page=8, pages=14)
+    out = t.prefill([tok, pos], cache, counts=counts)
+    for b, c in enumerate(counts):
+        if c:
+            near(out[b, :c], want[b, :c], dev)
+    assert cache.lengths.tolist() == counts
+    # the next token of each row: the sequence as if the padding had never been there
+    at = torch.tensor(counts, device=dev)
+    nxt, npos = (at + 3) % VOCAB, at + VOCAB
+    got = t.decode([nxt, npos], cache)
+    for b, c in enumerate(counts):
+        one = [torch.cat([tok[b, :c], nxt[b:b + 1]])[None], torch.cat([pos[b, :c], npos[b:b + 1]])[None]]
+        with torch.no_grad():
+            near(got[b], t(one)[0][0, -1], dev)
+    # row 2 leaves and another prompt takes its place; the others go on undisturbed
+    cache.release([2])
+    assert cache.lengths.tolist() == [31, 2, 0, 1]
+    tok2, pos2 = ids(1, 12, dev, first=0)
+    t.prefill([tok2, pos2], cache, rows=[2])
+    assert cache.lengths.tolist() == [31, 2, 12, 1] and cache.seen.tolist() == [31, 2, 12, 1]
+    got = t.decode([nxt, npos + 1], cache)
+    with torch.no_grad():
+        near(got[0], t([torch.cat([tok[0], nxt[:1], nxt[:1]])[None], torch.cat([pos[0], npos[:1], npos[:1] + 1])[None]])[0][0, -1], dev)
+        near(got[2], t([torch.cat([tok2[0], nxt[2:3]])[None], torch.cat([pos2[0], npos[2:3] + 1])[None]])[0][0, -1], dev)
+    # the book: no page in two rows
+    used = [p for own in cache._pages for p in own]
+    assert len(used) == len(set(used)) and not set(used) & set(cache._free) and len(used) + len(cache._free) == 14
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("slack", [0, 5])
+def test_eviction_while_decoding(dev, slack):
+    """Every head keeps its recent tokens, and its keys and values stay with their positions; a cache
+    that never reaches its budget changes nothing."""
+    t = layer(dev, blocks=1)
+    tok, pos = ids(2, 40, dev)
+    free, tight = t.init_cache(2, page=8), t.init_cache(2, page=8, budget=16, recent=6, slack=slack)
+    loose = t.init_cache(2, page=8, budget=48)
+    for c in (free, tight, loose):
+        t.prefill([tok[:, :20], pos[:, :20]], c)
+    for i in range(20, 40):
+        a, b, _ = (t.decode([tok[:, i], pos[:, i]], c) for c in (free, loose, tight))
+        assert torch.equal(a, b)
+    n = tight.lengths.tolist()
+    assert n[0] == n[1] and 16 <= n[0] <= 16 + slack and tight.seen.tolist() == [40, 40]
+    assert len(tight._pages[0]) <= -(-(16 + slack + 1) // 8)
+    kf, vf, _, _ = free.layer(0)
+    kt, vt, scores, positions = tight.layer(0)
+    for b in range(2):
+        for h in range(4):
+            rows = [(int(tight.page_table[b, s // 8]), s % 8) for s in range(n[b])]
+            held = [int(positions[p, h, r]) for p, r in rows]
+            assert len(set(held)) == n[b] and set(range(34, 40)) <= set(held)
+            for (p, r), x in zip(rows, held):
+                q = int(free.page_table[b, x // 8])
+                assert torch.equal(kt[p, h, r], kf[q, h, x % 8]) and torch.equal(vt[p, h, r], vf[q, h, x % 8])
+    # the weights of a step sum to one for each of the heads
+    total = torch.stack([torch.stack([loose.scores[int(loose.page_table[b, s // 8]), :, s % 8] for s in range(40)]).sum(0)
+                         for b in range(2)])
+    assert torch.allclose(total, torch.full_like(total, 20.0), atol=20 * 40 * 2.0 ** -20)
+
+
+def test_refusals():
+    t = layer("cpu")
+    tok, pos = ids(2, 10, "cpu")
+    cache = t.init_cache(2, max_length=12, page=4, pages=5)
+    with pytest.raises(RuntimeError, match="no pages left"):
+        t.prefill([tok, pos], cache)
+    assert cache.lengths.tolist() == [0, 0] and len(cache._free) == 5
+    t.prefill([tok, pos], cache, counts=[10, 5])
+    with pytest.raises(RuntimeError, match="in use"):
+        t.prefill([tok, pos], cache, counts=[1, 1])
+    t.decode([tok[:, 0], pos[:, 0]], cache)
+    t.decode([tok[:, 0], pos[:, 0]], cache)
+    with pytest.raises(RuntimeError, match="max_length"):
+        t.decode([tok[:, 0], pos[:, 0]], cache)
+    with pytest.raises(ValueError):
+        t.decode([tok, pos], cache)
+    with pytest.raises(ValueError):
+        t.prefill([tok, pos], cache, rows=[0])
+    with pytest.raises(ValueError):
+        t.prefill([tok, pos], t.init_cache(2), counts=[11, 1])
+    for bad in (dict(budget=0), dict(budget=4, recent=5), dict(recent=2), dict(slack=1), dict(page=0)):
+        with pytest.raises(ValueError):
+            t.init_cache(2, **bad)
+    t.train()
+    with pytest.raises(RuntimeError, match="eval"):
+        t.prefill([tok, pos], t.init_cache(2))
+    both = TransformerLayer.init(vocab=80, seq_len=8, n_block=1, hidden_size=16, n_head=2, bidirectional=True).eval()
+    with pytest.raises(RuntimeError, match="bidirectional"):
+        both.prefill([tok % 8, pos % 8], both.init_cache(2, max_length=12))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("budget", [None, 24])
+def test_captured_steps(gpu, budget):
+    """A captured decoding step, replayed with other work between the replays, does what the eager one does, bit for bit."""
+    t = layer("cuda", blocks=2)
+    tok, pos = ids(3, 60, "cuda")
+    caches = [t.init_cache(3, max_length=80, page=16, budget=budget, recent=8 if budget else None) for _ in range(2)]
+    start = 30
+    for c in caches:
+        t.prefill([tok[:, :start], pos[:, :start]], c)
+        t.decode([tok[:, start], pos[:, start]], c)
+        c.reserve(30)
+    eager, static = caches
+    x, p = tok[:, start + 1].clone(), pos[:, start + 1].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    spare = t.init_cache(3, max_length=80, page=16, budget=budget)
+    with torch.cuda.stream(side):
+        t.prefill([tok[:, :4], pos[:, :4]], spare)
+        t.decode([x, p], spare)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = t.decode([x, p], static)
+    for i in range(start + 1, 55):
+        x.copy_(tok[:, i])
+        p.copy_(pos[:, i])
+        g.replay()
+        if i > start + 1:
+            static.replayed(1, evicts=budget is not None)
+        junk = torch.randn(512, 512, device="cuda") @ torch.randn(512, 512, device="cuda")
+        want = t.decode([tok[:, i], pos[:, i]], eager)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), i
+        assert torch.equal(static.lengths, eager.lengths) and torch.equal(static.seen, eager.seen)
+    assert static._slots == eager._slots
+    assert torch.isfinite(junk).all()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once_and_another_stream(gpu):
+    """Two sequences of calls on two streams at the same time: each call's workspace is its own."""
+    from test_kvcache import make
+    args = [make(4, 2, 4, 128, 64, [3000, 700, 0, 2049], torch.bfloat16, "cuda", seed=s) for s in range(2)]
+    want = [paged_attention(*a) for a in args]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(paged_attention(*args[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+@pytest.mark.gpu
+def test_a_step_by_hand(gpu):
+    """Append, attend and evict through zoo.ops alone, lengths updated in place, against the CPU implementation."""
+    out = {}
+    for dev in ("cpu", "cuda"):
+        g = torch.Generator().manual_seed(9)
+        k, v = (torch.zeros(12, 2, 8, 16).to(dev) for _ in range(2))
+        scores, positions = torch.zeros(12, 2, 8).to(dev), torch.zeros(12, 2, 8, dtype=torch.int32).to(dev)
+        table = torch.tensor([[3, 1, 7, 5], [0, 11, 2, 9]], dtype=torch.int32).to(dev)
+        n = torch.zeros(2, dtype=torch.int32).to(dev)
+        seen = n.clone()
+        outs = []
+        for step in range(40):
+            kv = torch.randn(2, 1, 2, 2, 16, generator=g).to(dev)
+            q = torch.randn(2, 6, 16, generator=g).to(dev)
+            n.copy_(paged_append(kv[:, :, 0], kv[:, :, 1], k, v, table, n, seen=seen, scores=scores, positions=positions))
+            seen += 1
+            outs.append(paged_attention(q, k, v, table, n, scores=scores).cpu())
+            n.copy_(paged_evict(k, v, scores, positions, table, n, seen, 20, 4))
+        out[dev] = (torch.stack(outs), positions.cpu(), n.cpu())
+    # float32 sums in another order: 2^-24 times a few hundred additions
+    assert torch.allclose(out["cpu"][0], out["cuda"][0], atol=1e-5)
+    assert torch.equal(out["cpu"][1], out["cuda"][1]) and out["cpu"][2].tolist() == [20, 20] == out["cuda"][2].tolist()
+
+
+def test_the_book_on_its_own():
+    c = PagedKVCache(1, 2, 20, 1, 8, page=4, device="cpu")
+    c.reserve([20, 3])
+    assert (c.page_table >= 0).sum(1).tolist() == [5, 1]
+    c.release([0])
+    assert (c.page_table >= 0).sum(1).tolist() == [0, 1] and len(c._free) == 9
+    with pytest.raises(RuntimeError):
+        c.reserve(21)
+    with pytest.raises(RuntimeError):
+        c.replayed(5)
