@@ -7,6 +7,8 @@ namespace zoo {
 
 constexpr int kKvMaxGroup = 256;        // query heads that may share one kv head
 constexpr int kKvMaxSlots = 1 << 30;    // slots one sequence may name
+constexpr int kEvictHeld = 16384;       // slots of a row that one workgroup selects from, its keys in LDS
+constexpr int kEvictSeg = 1024;         // slots of a workgroup where a row is shared out
 constexpr int kEvictRow = 16 + 3 * 2048;  // ints of a row's selection state where it is shared out
 
 // unsigned n / d for n < 2^31 as (mulhi(n, m) + n) >> s (Granlund and Montgomery's round-up method)
@@ -28,7 +30,7 @@ struct PagedAttnArgs {
   const float* scores;       // pools [pages, H, page], or null: no weights wanted
   float* scores_out;
   void* o;                   // [B, H * G, D]
-  float* logits;             // [B, H, cap, G] raw products q.k (weights only)
+  float* logits;             // [B, H * G, pitch] raw products q.k (weights only)
   float* part_o;             // [items, gs, D] partial sums of a split sequence
   float* part_ml;            // [items, 16, 2] their running maximum (log2 units) and sum
   int4* plan;                // [items, 2] who does what, for the join; null where there is none
@@ -36,6 +38,7 @@ struct PagedAttnArgs {
   PoolStride ks, vs, ss, sos;
   FastDiv page;
   int B, H, G, D, pages, cap;
+  int pitch;                 // cap rounded up to 16
   int dtype;                 // 0 bf16, 1 fp16, 2 fp32
   int gs;                    // min(G, 16)
   int single;                // 1: every sequence is one work item

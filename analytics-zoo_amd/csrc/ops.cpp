@@ -3220,6 +3220,7 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   TORCH_CHECK(items < (1LL << 31), what, ": too many heads in the batch");
   auto f32 = q.options().dtype(at::kFloat);
   torch::Tensor ml, po, logits, plan;
+  const int64_t pitch = (c.cap + 15) / 16 * 16;
   const int64_t gs = std::min<int64_t>(G, 16);
   if (!a.single || (weights && G > 16)) {
     ml = torch::empty({items, 16, 2}, f32);
@@ -3227,7 +3228,7 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
     a.plan = reinterpret_cast<int4*>(plan.data_ptr<int>());
   }
   if (!a.single) po = torch::empty({items, gs, c.D}, f32);
-  if (weights) logits = torch::empty({c.B, c.H, c.cap, G}, f32);
+  if (weights) logits = torch::empty({c.B, c.H * G, pitch}, f32);
   a.q = q.data_ptr(), a.k = kp.data_ptr(), a.v = vp.data_ptr();
   a.table = table.data_ptr<int>(), a.len = lengths.data_ptr<int>();
   a.o = o.data_ptr();
@@ -3241,7 +3242,7 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   a.q_b = q.stride(0), a.q_h = q.stride(1), a.table_b = table.stride(0);
   a.ks = pool_stride(kp), a.vs = pool_stride(vp);
   a.page = fast_div((uint32_t)c.page);
-  a.B = c.B, a.H = c.H, a.G = G, a.D = c.D, a.pages = c.P, a.cap = c.cap, a.dtype = c.dtype, a.gs = gs;
+  a.B = c.B, a.H = c.H, a.G = G, a.D = c.D, a.pages = c.P, a.cap = c.cap, a.pitch = pitch, a.dtype = c.dtype, a.gs = gs;
   a.hbs = hbs, a.step = fast_div((uint32_t)per_seq);
   a.per_target = (float)(0.999 / target), a.at_once = at_once >= c.B ? at_once : 0;
   a.c = (float)(scale * 1.4426950408889634);
@@ -3331,7 +3332,7 @@ torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scor
   a.page = fast_div((uint32_t)c.page), a.vec = fast_div((uint32_t)vec);
   a.B = c.B, a.H = c.H, a.pages = c.P, a.cap = c.cap, a.es = c.es;
   a.budget = budget, a.recent = recent, a.most = most;
-  a.segs = c.cap > 16384 ? (c.cap + 4095) / 4096 : 0;
+  a.segs = c.cap > zoo::kEvictHeld ? (c.cap + zoo::kEvictSeg - 1) / zoo::kEvictSeg : 0;
   TORCH_CHECK(rows * std::max(a.segs, 1) < (1LL << 31), what, ": too many heads or slots in the batch");
   torch::Tensor hist, keys;
   if (a.segs > 0) {

@@ -338,6 +338,10 @@ def test_evict_long(gpu, H, D, page, dtype, order, lengths, budget, recent, kind
     (1, 8, 128, BF, "phsd", [2500], 2048, 0, "zeros"),
     (2, 8, 16, FL, "phsd", [300], 100, 50, "twice"),
     (1, 8, 16, FL, "phsd", [30], 1000, 3, "plain"),
+    (2, 8, 16, FL, "phsd", [24, 23, 22, 21, 25], 20, 0, "ties"),      # a few over the budget
+    (2, 8, 16, FL, "phsd", [104, 103, 102, 101, 105], 100, 9, "zeros"),
+    (3, 8, 5, FL, "pshd", [3, 4, 5, 2], 1, 0, "odd"),
+    (1, 8, 64, BF, "phsd", [3003, 3001], 3000, 3000, "odd"),
 ])
 def test_evict(dev, H, D, page, dtype, order, lengths, budget, recent, kind):
     B = len(lengths)
