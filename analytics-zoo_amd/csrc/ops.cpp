@@ -3217,7 +3217,7 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   zoo::PagedAttnArgs a{};
   a.single = c.cap * c.D * c.es * 2 <= 256 * 1024;
   const int64_t items = (a.single ? c.B : c.B + target + target / 512 + 1) * per_seq;
-  TORCH_CHECK(items < (1LL << 31), what, ": too many heads in the batch");
+  TORCH_CHECK(items < (1LL << 23), what, ": too many heads in the batch");    // 512 threads each, below 2^32
   auto f32 = q.options().dtype(at::kFloat);
   torch::Tensor ml, po, logits, plan;
   const int64_t pitch = (c.cap + 15) / 16 * 16;
@@ -3264,8 +3264,8 @@ torch::Tensor paged_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, t
   }
   TORCH_CHECK(k.size(1) == v.size(1), what, ": k and v have other numbers of tokens");
   const int64_t T = k.size(1), vec = c.D * c.es / 16;
-  TORCH_CHECK(T * c.H * vec < (1LL << 31) - 256 && c.B * ((T * c.H * vec + 255) / 256 + 1) < (1LL << 31), what,
-              ": too many tokens in one call");
+  TORCH_CHECK(T * c.H * vec < (1LL << 31) - 256 && c.B * ((T * c.H * vec + 255) / 256 + 1) < (1LL << 24), what,
+              ": too many tokens in one call");    // below 2^32 threads
   paged_written(kp, vp);
   if (counts.has_value()) paged_ints(*counts, lengths, "counts", what);
   if (seen.has_value()) paged_ints(*seen, lengths, "seen", what);
@@ -3316,8 +3316,7 @@ torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scor
   if (c.B == 0) return len_out;
   const int64_t vec = c.D * c.es / 16, rows = c.B * c.H;
   const int64_t most = std::max<int64_t>(0, std::min(budget, c.cap - budget));
-  TORCH_CHECK(rows * ((most * vec + 255) / 256 + 1) < (1LL << 31) && most * vec < (1LL << 31) - 256, what,
-              ": too many heads or slots in the batch");
+  TORCH_CHECK(rows < (1LL << 22) && most * vec < (1LL << 30), what, ": too many heads or slots in the batch");
   auto moves = torch::empty({rows * (2 * most + 1)}, lengths.options());
   zoo::PagedEvictArgs a{};
   a.kp = kp.data_ptr(), a.vp = vp.data_ptr();
@@ -3333,7 +3332,7 @@ torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scor
   a.B = c.B, a.H = c.H, a.pages = c.P, a.cap = c.cap, a.es = c.es;
   a.budget = budget, a.recent = recent, a.most = most;
   a.segs = c.cap > zoo::kEvictHeld ? (c.cap + zoo::kEvictSeg - 1) / zoo::kEvictSeg : 0;
-  TORCH_CHECK(rows * std::max(a.segs, 1) < (1LL << 31), what, ": too many heads or slots in the batch");
+  TORCH_CHECK(rows * std::max(a.segs, 1) < (1LL << 24), what, ": too many heads or slots in the batch");
   torch::Tensor hist, keys;
   if (a.segs > 0) {
     hist = torch::zeros({(int64_t)zoo_paged_evict_scratch(&a)}, lengths.options());

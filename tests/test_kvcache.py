@@ -428,3 +428,65 @@ def test_refusals(dev):
         no(paged_append, x, x, k[:1].expand(k.shape), v, table, n)
         no(paged_evict, k, v, s.half(), p, table, n, n, 4)
         no(paged_evict, k, v, s, p.long(), table, n, n, 4)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("pages,batch,width", [(0, 2, 3), (4, 2, 0), (4, 0, 3), (0, 0, 0)])
+def test_nothing_there(dev, pages, batch, width):
+    """No pages, no sequences, no room in the table: empty sequences are zeros, and there are no others."""
+    k, v = (torch.zeros(pages, 2, 8, 16).to(dev) for _ in range(2))
+    s, p = torch.zeros(pages, 2, 8).to(dev), torch.zeros(pages, 2, 8, dtype=torch.int32).to(dev)
+    table = torch.zeros(batch, width, dtype=torch.int32).to(dev)
+    n = torch.zeros(batch, dtype=torch.int32).to(dev)
+    q, new = torch.ones(batch, 4, 16).to(dev), torch.ones(batch, 1, 2, 16).to(dev)
+    o = paged_attention(q, k, v, table, n)
+    assert tuple(o.shape) == (batch, 4, 16) and not o.any()
+    assert not paged_attention(q, k, v, table, n, scores=s).any()
+    assert paged_evict(k, v, s, p, table, n, n.clone(), 3, 1).tolist() == [0] * batch
+    after = paged_append(new, new, k, v, table, n, scores=s, positions=p)
+    assert after.tolist() == [1] * batch
+    if batch and (width == 0 or pages == 0):
+        assert torch.isnan(paged_attention(q, k, v, table, after)).all()
+        assert paged_evict(k, v, s, p, table, after, after.clone(), 3, 1).tolist() == [1] * batch
+
+
+@GPU
+def test_far_pages(gpu):
+    """Offsets past 2^31 elements and 2^32 bytes: the last pages of a pool of 5 GiB."""
+    P = 5 * 2 ** 30 // (2 * 128 * 128 * 2)
+    k = torch.zeros(P, 2, 128, 128, dtype=BF, device="cuda")
+    assert k.numel() > 2 ** 31
+    near = make(2, 2, 2, 128, 128, [300, 129], BF, "cuda")
+    q, kn, vn, table, n = near
+    v = torch.zeros_like(k)
+    far = torch.where(table >= 0, table + (P - kn.shape[0]), table)
+    k[P - kn.shape[0]:], v[P - kn.shape[0]:] = kn, vn
+    assert torch.equal(paged_attention(q, k, v, far, n), paged_attention(q, kn, vn, table, n))
+    new = torch.randn(2, 3, 2, 128).to(BF).cuda()
+    for kk, vv, t in ((k, v, far), (kn, vn, table)):
+        s = torch.arange(128, device="cuda").expand(kk.shape[:3]).remainder(37).float().contiguous()
+        p = torch.zeros(kk.shape[:3], dtype=torch.int32, device="cuda")
+        m = paged_append(new, new, kk, vv, t, n, scores=s, positions=p)
+        paged_evict(kk, vv, s, p, t, m, m + 1000, 100, 0)
+    a, b = k[P - kn.shape[0]:], v[P - kn.shape[0]:]
+    assert torch.equal(a.nan_to_num(), kn.nan_to_num()) and torch.equal(b.nan_to_num(), vn.nan_to_num())
+    assert not k[:P - kn.shape[0]].any()
+
+
+@GPU
+def test_many_short_sequences(gpu):
+    """More sequences than a wave has lanes, split and unsplit, with bad ones among them."""
+    g = torch.Generator().manual_seed(4)
+    lengths = torch.randint(0, 900, (300,), generator=g).tolist()
+    q, k, v, table, n = make(300, 1, 2, 64, 32, lengths, BF, "cuda")
+    o = paged_attention(q, k, v, table, n)
+    wide = torch.nn.functional.pad(table, (0, 400), value=-1).contiguous()       # capacity past the unsplit form
+    n[7], n[200] = -5, 10 ** 6
+    o2 = paged_attention(q, k, v, wide, n)
+    assert torch.isnan(o2[[7, 200]]).all()
+    fine = [i for i in range(300) if i not in (7, 200)]
+    for b in (0, 63, 64, 128, 255, 299):
+        ref, mag, _ = define(q[b:b + 1], k, v, table[b:b + 1], lengths[b:b + 1])
+        close(o[b:b + 1], ref, mag, 64)
+        close(o2[b:b + 1], ref, mag, 64)
+    assert torch.isfinite(o2[fine]).all()
