@@ -30,13 +30,29 @@
 // chunks and, where weights are wanted, turns the stored products into sum_g w_gj.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 #include "kvcache.h"
 
 namespace zoo {
 namespace {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// NT: past the caches, for what will not be read again before it would have left them anyway
+template <bool NT>
+ZOO_DEV uint4 load16(const void* p) {
+  if constexpr (NT) return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const u32x4*)p));
+  return *(const uint4*)p;
+}
+template <bool NT>
+ZOO_DEV uint2 load8(const void* p) {
+  if constexpr (NT) return __builtin_bit_cast(uint2, __builtin_nontemporal_load((const u32x2*)p));
+  return *(const uint2*)p;
+}
 
 enum { kBf16 = 0, kF16 = 1, kF32 = 2 };
 
@@ -87,6 +103,7 @@ struct Work {
   int s0, s1;       // its slots
   int len;          // the sequence's slots, -1: bad
   int first;        // item of the sequence's chunk 0, same head block
+  bool big;         // the batch's keys and values do not fit the last-level cache
 };
 
 ZOO_DEV int chunks_of(int len, int size) { return len <= size ? 1 : (int)(((unsigned)len + size - 1) / (unsigned)size); }
@@ -116,7 +133,7 @@ ZOO_DEV bool find_work(const PagedAttnArgs& a, int grain, Work& w) {
   w.hb = 0, w.hk = hh;
   if (a.hbs > 1) w.hk = hh / a.hbs, w.hb = hh - w.hk * a.hbs;
   if (a.single) {
-    w.b = uni(t), w.chunk = 0, w.n = 1, w.first = item;
+    w.b = uni(t), w.chunk = 0, w.n = 1, w.first = item, w.big = false;
     w.len = seq_len(a.len, w.b, a.cap);
     w.s0 = 0, w.s1 = w.len;
     return true;
@@ -125,6 +142,7 @@ ZOO_DEV bool find_work(const PagedAttnArgs& a, int grain, Work& w) {
   float total = (float)max(mine0, 0);
   for (int b = lane + 64; b < a.B; b += 64) total += (float)max(seq_len(a.len, b, a.cap), 0);
   total = wave_total(total);
+  w.big = total > a.cached;
   // per_target is 0.999 / target, so that a total that divides evenly is not rounded up to another grain
   int size = chunk_size(total * a.per_target, grain);
   // Sequences end inside chunks, so there are more chunks than the total asks for: if they would
@@ -291,7 +309,7 @@ ZOO_DEV void gather_weights(const PagedAttnArgs& a, int b, int hk, int s0, int s
 // 16-slot subtile lies in one page and its address is wave-uniform. Other page sizes look up a page per
 // slot.
 template <int DT, int DP, bool PAD, bool P16>
-__global__ __launch_bounds__(256, DP == 256 ? (DT == kF32 ? 1 : 2) : DT == kF32 && DP == 128 && PAD ? 2 : 3) void paged_attn_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD ? 2 : 3) void paged_attn_kernel(const PagedAttnArgs a) {
   using T = Tile<DT, DP>;
   constexpr int NS = T::NS, KL = T::KL, VC = T::VC, VW = T::VW, VE = T::VE, NA = T::NA, ES = T::ES;
   extern __shared__ float lds[];  // [4][gb][DP + 4] sums, then [4][16][2] maximum and sum
@@ -347,7 +365,8 @@ __global__ __launch_bounds__(256, DP == 256 ? (DT == kF32 ? 1 : 2) : DT == kF32 
     bad |= !ok;
     return ok ? p : 0;
   };
-  auto load_k = [&](int base) {
+  auto load_k = [&](int base, auto nt) {
+    constexpr bool NT = decltype(nt)::value;
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
       const char* p;
@@ -362,14 +381,15 @@ __global__ __launch_bounds__(256, DP == 256 ? (DT == kF32 ? 1 : 2) : DT == kF32 
       for (int i = 0; i < KL; ++i) {
         if constexpr (PAD) {
           const bool in = i * 64 + quad * 16 < D * ES;
-          kr[u][i] = mask4(*(const uint4*)(p + (in ? i * 64 : -quad * 16)), in);
+          kr[u][i] = mask4(load16<NT>(p + (in ? i * 64 : -quad * 16)), in);
         } else {
-          kr[u][i] = *(const uint4*)(p + i * 64);
+          kr[u][i] = load16<NT>(p + i * 64);
         }
       }
     }
   };
-  auto load_v = [&](int base) {
+  auto load_v = [&](int base, auto nt) {
+    constexpr bool NT = decltype(nt)::value;
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
       const char* p0 = vb;
@@ -391,10 +411,10 @@ __global__ __launch_bounds__(256, DP == 256 ? (DT == kF32 ? 1 : 2) : DT == kF32 
           const int at = c * 256 + vdim;
           const char* pc = p + (!PAD || at < D * ES ? at : 0);
           if constexpr (VW == 4) {
-            const uint4 x = *(const uint4*)pc;
+            const uint4 x = load16<NT>(pc);
             vr[u][r][c][0] = x.x, vr[u][r][c][1] = x.y, vr[u][r][c][2] = x.z, vr[u][r][c][3] = x.w;
           } else {
-            const uint2 x = *(const uint2*)pc;
+            const uint2 x = load8<NT>(pc);
             vr[u][r][c][0] = x.x, vr[u][r][c][1] = x.y;
           }
         }
@@ -408,113 +428,119 @@ __global__ __launch_bounds__(256, DP == 256 ? (DT == kF32 ? 1 : 2) : DT == kF32 
   float m = -INFINITY, l = 0.f;  // of head `row`; l of this lane's slots only
   float* logit = a.logits ? a.logits + ((long)w.b * a.H * a.G + head0 + row) * a.pitch + 4 * quad : nullptr;
 
-  int base = w.s0 + wave * T::TS;
-  if (base < w.s1) {
-    load_k(base);
-    load_v(base);
-  }
-  for (; base < w.s1; base += T::GRAIN) {
-    const bool more = base + T::GRAIN < w.s1, tail = base + T::TS > w.s1;
-    f32x4 s[NS];
+  auto stream = [&](auto nt) {
+    int base = w.s0 + wave * T::TS;
+    if (base < w.s1) {
+      load_k(base, nt);
+      load_v(base, nt);
+    }
+    for (; base < w.s1; base += T::GRAIN) {
+      const bool more = base + T::GRAIN < w.s1, tail = base + T::TS > w.s1;
+      f32x4 s[NS];
 #pragma unroll
-    for (int u = 0; u < NS; ++u) {
-      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < NS; ++u) {
+        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        if constexpr (DT == kF32) {
-          s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].x), __uint_as_float(q[i].x), s[u], 0, 0, 0);
-          s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].y), __uint_as_float(q[i].y), s[u], 0, 0, 0);
-          s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].z), __uint_as_float(q[i].z), s[u], 0, 0, 0);
-          s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].w), __uint_as_float(q[i].w), s[u], 0, 0, 0);
-        } else {
-          s[u] = mma16<DT>(kr[u][i], q[i], s[u]);
+        for (int i = 0; i < KL; ++i) {
+          if constexpr (DT == kF32) {
+            s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].x), __uint_as_float(q[i].x), s[u], 0, 0, 0);
+            s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].y), __uint_as_float(q[i].y), s[u], 0, 0, 0);
+            s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].z), __uint_as_float(q[i].z), s[u], 0, 0, 0);
+            s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].w), __uint_as_float(q[i].w), s[u], 0, 0, 0);
+          } else {
+            s[u] = mma16<DT>(kr[u][i], q[i], s[u]);
+          }
         }
       }
-    }
-    if (more) load_k(base + T::GRAIN);
-    if (logit != nullptr && row < gb) {
-      // rows are padded to whole subtiles, so 4 slots go at once
+      if (more) load_k(base + T::GRAIN, nt);
+      if (logit != nullptr && row < gb) {
+        // rows are padded to whole subtiles, so 4 slots go at once
 #pragma unroll
-      for (int u = 0; u < NS; ++u)
-        if (base + 16 * u < w.s1) *(f32x4*)(logit + base + 16 * u) = s[u];
-    }
-    float top = m;
-#pragma unroll
-    for (int u = 0; u < NS; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[u][r] *= a.c;
-        if (tail && base + 16 * u + 4 * quad + r >= w.s1) s[u][r] = -INFINITY;
-        top = fmaxf(top, s[u][r]);
+        for (int u = 0; u < NS; ++u)
+          if (base + 16 * u < w.s1) *(f32x4*)(logit + base + 16 * u) = s[u];
       }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float mu = top == -INFINITY ? 0.f : top;  // nothing but -inf so far: every weight is 0, not NaN
-    const float old = pow2(m - mu);
-    m = top;
-    l *= old;
-    if (__any(old != 1.f)) {
-#pragma unroll
-      for (int i = 0; i < NA; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][r] *= old;
-    }
-#pragma unroll
-    for (int u = 0; u < NS; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[u][r] = pow2(s[u][r] - mu + kUp);
-        l += s[u][r];
-      }
-    // a slot behind the last has weight 0, but 0 times what its row happens to hold may be NaN
-    if (tail) {
+      float top = m;
 #pragma unroll
       for (int u = 0; u < NS; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const uint32_t keep = base + 16 * u + 4 * quad + r < w.s1 ? 0xffffffffu : 0u;
-#pragma unroll
-          for (int c = 0; c < VC; ++c)
-#pragma unroll
-            for (int i = 0; i < VW; ++i) vr[u][r][c][i] &= keep;
+          s[u][r] *= a.c;
+          if (tail && base + 16 * u + 4 * quad + r >= w.s1) s[u][r] = -INFINITY;
+          top = fmaxf(top, s[u][r]);
         }
-    }
-    if constexpr (DT == kF32) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float mu = top == -INFINITY ? 0.f : top;  // nothing but -inf so far: every weight is 0, not NaN
+      const float old = pow2(m - mu);
+      m = top;
+      l *= old;
+      if (__any(old != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][r] *= old;
+      }
 #pragma unroll
       for (int u = 0; u < NS; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r) {
+          s[u][r] = pow2(s[u][r] - mu + kUp);
+          l += s[u][r];
+        }
+      // a slot behind the last has weight 0, but 0 times what its row happens to hold may be NaN
+      if (tail) {
+#pragma unroll
+        for (int u = 0; u < NS; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t keep = base + 16 * u + 4 * quad + r < w.s1 ? 0xffffffffu : 0u;
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+              for (int i = 0; i < VW; ++i) vr[u][r][c][i] &= keep;
+          }
+      }
+      if constexpr (DT == kF32) {
+#pragma unroll
+        for (int u = 0; u < NS; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+              for (int e = 0; e < VE; ++e)
+                acc[c * VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[u][r][c][e]), s[u][r],
+                                                                       acc[c * VE + e], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int u = 0; u < NS; u += 2) {
+          uint4 hi, lo;
+          split2<DT>(s[u][0], s[u][1], hi.x, lo.x);
+          split2<DT>(s[u][2], s[u][3], hi.y, lo.y);
+          split2<DT>(s[u + 1][0], s[u + 1][1], hi.z, lo.z);
+          split2<DT>(s[u + 1][2], s[u + 1][3], hi.w, lo.w);
 #pragma unroll
           for (int c = 0; c < VC; ++c)
 #pragma unroll
-            for (int e = 0; e < VE; ++e)
-              acc[c * VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[u][r][c][e]), s[u][r],
-                                                                     acc[c * VE + e], 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int u = 0; u < NS; u += 2) {
-        uint4 hi, lo;
-        split2<DT>(s[u][0], s[u][1], hi.x, lo.x);
-        split2<DT>(s[u][2], s[u][3], hi.y, lo.y);
-        split2<DT>(s[u + 1][0], s[u + 1][1], hi.z, lo.z);
-        split2<DT>(s[u + 1][2], s[u + 1][3], hi.w, lo.w);
-#pragma unroll
-        for (int c = 0; c < VC; ++c)
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-            uint4 x;
-            x.x = __builtin_amdgcn_perm(vr[u][1][c][e / 2], vr[u][0][c][e / 2], sel);
-            x.y = __builtin_amdgcn_perm(vr[u][3][c][e / 2], vr[u][2][c][e / 2], sel);
-            x.z = __builtin_amdgcn_perm(vr[u + 1][1][c][e / 2], vr[u + 1][0][c][e / 2], sel);
-            x.w = __builtin_amdgcn_perm(vr[u + 1][3][c][e / 2], vr[u + 1][2][c][e / 2], sel);
-            acc[c * VE + e] = mma16<DT>(x, hi, acc[c * VE + e]);
-            acc[c * VE + e] = mma16<DT>(x, lo, acc[c * VE + e]);
-          }
+            for (int e = 0; e < VE; ++e) {
+              const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+              uint4 x;
+              x.x = __builtin_amdgcn_perm(vr[u][1][c][e / 2], vr[u][0][c][e / 2], sel);
+              x.y = __builtin_amdgcn_perm(vr[u][3][c][e / 2], vr[u][2][c][e / 2], sel);
+              x.z = __builtin_amdgcn_perm(vr[u + 1][1][c][e / 2], vr[u + 1][0][c][e / 2], sel);
+              x.w = __builtin_amdgcn_perm(vr[u + 1][3][c][e / 2], vr[u + 1][2][c][e / 2], sel);
+              acc[c * VE + e] = mma16<DT>(x, hi, acc[c * VE + e]);
+              acc[c * VE + e] = mma16<DT>(x, lo, acc[c * VE + e]);
+            }
+        }
       }
+      if (more) load_v(base + T::GRAIN, nt);
     }
-    if (more) load_v(base + T::GRAIN);
-  }
+  };
+  if (P16 && !PAD && w.big)
+    stream(std::bool_constant<P16 && !PAD>{});
+  else
+    stream(std::false_type{});
   const bool weights = w.n == 1 && a.logits != nullptr && a.G <= 16;
   Ahead ahead;
   if (weights && threadIdx.x < w.s1) ahead = weights_ahead(a, w.b, w.hk, threadIdx.x, w.s1);
@@ -659,8 +685,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
   const int pi = fdiv(slot, a.page), p = a.table[b * a.table_b + pi];
   if ((unsigned)p >= (unsigned)a.pages) return;
   const long off = slot - pi * a.page.d;
-  const uint4 x = *(const uint4*)((const char*)a.k + (b * a.k_b + t * a.k_t + h * a.k_h) * a.es + piece * 16);
-  const uint4 y = *(const uint4*)((const char*)a.v + (b * a.v_b + t * a.v_t + h * a.v_h) * a.es + piece * 16);
+  const uint4 x = load16<true>((const char*)a.k + (b * a.k_b + t * a.k_t + h * a.k_h) * a.es + piece * 16);
+  const uint4 y = load16<true>((const char*)a.v + (b * a.v_b + t * a.v_t + h * a.v_h) * a.es + piece * 16);
   *(uint4*)((char*)a.kp + (p * a.ks.page + h * a.ks.head + off * a.ks.row) * a.es + piece * 16) = x;
   *(uint4*)((char*)a.vp + (p * a.vs.page + h * a.vs.head + off * a.vs.row) * a.es + piece * 16) = y;
   if (piece == 0) {
@@ -1059,8 +1085,8 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(const PagedEvictA
     const long piece = (i - n * a.vec.d) * 16;
     const int to = give[n], from = give[a.most + n];
     const int tp = row.id(to), fp = row.id(from);
-    const uint4 x = *(const uint4*)(kp + row.at(from, fp, a.ks) * a.es + piece);
-    const uint4 y = *(const uint4*)(vp + row.at(from, fp, a.vs) * a.es + piece);
+    const uint4 x = load16<true>(kp + row.at(from, fp, a.ks) * a.es + piece);
+    const uint4 y = load16<true>(vp + row.at(from, fp, a.vs) * a.es + piece);
     *(uint4*)(kp + row.at(to, tp, a.ks) * a.es + piece) = x;
     *(uint4*)(vp + row.at(to, tp, a.vs) * a.es + piece) = y;
     if (piece == 0) {
