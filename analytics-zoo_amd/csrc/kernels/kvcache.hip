@@ -884,6 +884,28 @@ ZOO_DEV bool each_key(const PagedEvictArgs& a, const Row& row, int s0, int s1, l
   return bad;
 }
 
+// Moves the n slots that the lists of row r say, 16 bytes of a key row and of a value row at a time: the pieces first,
+// first + step, ..
+ZOO_DEV void move_rows(const PagedEvictArgs& a, const Row& row, int r, int n, uint32_t first, uint32_t step) {
+  const int* give = a.moves + (long)r * 2 * a.most;
+  const uint32_t total = (uint32_t)n * a.vec.d;
+  char *kp = (char*)a.kp, *vp = (char*)a.vp;
+  for (uint32_t i = first; i < total; i += step) {
+    const int m = fdiv(i, a.vec);
+    const long piece = (i - m * a.vec.d) * 16;
+    const int to = give[m], from = give[a.most + m];
+    const int tp = row.id(to), fp = row.id(from);
+    const uint4 x = load16<true>(kp + row.at(from, fp, a.ks) * a.es + piece);
+    const uint4 y = load16<true>(vp + row.at(from, fp, a.vs) * a.es + piece);
+    *(uint4*)(kp + row.at(to, tp, a.ks) * a.es + piece) = x;
+    *(uint4*)(vp + row.at(to, tp, a.vs) * a.es + piece) = y;
+    if (piece == 0) {
+      a.scores_out[row.at(to, tp, a.sos)] = a.scores[row.at(from, fp, a.ss)];
+      a.positions_out[row.at(to, tp, a.pos)] = a.positions[row.at(from, fp, a.ps)];
+    }
+  }
+}
+
 // One workgroup per row (sequence and kv head), its keys in LDS: a radix selection of the budget-th largest by
 // digits of 11, 11 and 10 bits, then the lists, each wave a stretch of the slots. Bound by its
 // barriers and the latency of its loads.
@@ -972,10 +994,14 @@ __global__ __launch_bounds__(NT) void paged_evict_select_kernel(const PagedEvict
   if (gone > 0) cut.ties = eq_all - gone;
   int* give = a.moves + (long)blockIdx.x * 2 * a.most;
   list_range(a, row, s0, s1, before, eq_lo, cut, give, give + a.most, masks + wave * ((len + NT - 1) / NT), key);
-  if (tid == 0) {
-    int gt = 0, eq = 0;   // as many are kept behind the budget as are given up below it
-    for (int i = 0; i < NT / 64; ++i) gt += counts[i].gt_hi, eq += counts[i].eq_hi;
-    a.count[blockIdx.x] = gt + min(max(cut.ties - eq_lo, 0), eq);
+  int gt = 0, eq = 0;   // as many are kept behind the budget as are given up below it
+  for (int i = 0; i < NT / 64; ++i) gt += counts[i].gt_hi, eq += counts[i].eq_hi;
+  const int n = gt + min(max(cut.ties - eq_lo, 0), eq);
+  if (a.fused) {
+    __syncthreads();
+    move_rows(a, row, blockIdx.x, n, tid, NT);
+  } else if (tid == 0) {
+    a.count[blockIdx.x] = n;
   }
 }
 
@@ -1072,28 +1098,12 @@ __global__ __launch_bounds__(256) void paged_evict_long_kernel(const PagedEvictA
   }
 }
 
-// Moves what the lists say, 16 bytes of a key row and of a value row to a thread at a time. Bound by HBM: 131k -> 16k
-// slots of 8 heads of 128 move 117 MB in 27 us, 4.3 TB/s (a large copy: 4.8).
+// The moves of a row by many workgroups. Bound by HBM: 131k -> 16k slots of 8 heads of 128 move 117 MB in 26 us, 4.5
+// TB/s (a large copy: 4.8).
 __global__ __launch_bounds__(256) void paged_evict_move_kernel(const PagedEvictArgs a, int blocks_per_row) {
-  const int r = blockIdx.x / blocks_per_row, b = r / a.H, h = r - b * a.H;
-  const int* give = a.moves + (long)r * 2 * a.most;
-  const Row row{a.table + (long)b * a.table_b, a.page, h};
-  const uint32_t total = (uint32_t)a.count[r] * a.vec.d;
-  char *kp = (char*)a.kp, *vp = (char*)a.vp;
-  for (uint32_t i = (blockIdx.x - r * blocks_per_row) * 256 + threadIdx.x; i < total; i += blocks_per_row * 256) {
-    const int n = fdiv(i, a.vec);
-    const long piece = (i - n * a.vec.d) * 16;
-    const int to = give[n], from = give[a.most + n];
-    const int tp = row.id(to), fp = row.id(from);
-    const uint4 x = load16<true>(kp + row.at(from, fp, a.ks) * a.es + piece);
-    const uint4 y = load16<true>(vp + row.at(from, fp, a.vs) * a.es + piece);
-    *(uint4*)(kp + row.at(to, tp, a.ks) * a.es + piece) = x;
-    *(uint4*)(vp + row.at(to, tp, a.vs) * a.es + piece) = y;
-    if (piece == 0) {
-      a.scores_out[row.at(to, tp, a.sos)] = a.scores[row.at(from, fp, a.ss)];
-      a.positions_out[row.at(to, tp, a.pos)] = a.positions[row.at(from, fp, a.ps)];
-    }
-  }
+  const int r = blockIdx.x / blocks_per_row, b = r / a.H;
+  const Row row{a.table + (long)b * a.table_b, a.page, r - b * a.H};
+  move_rows(a, row, r, a.count[r], (blockIdx.x - r * blocks_per_row) * 256 + threadIdx.x, blocks_per_row * 256);
 }
 
 template <int DT, int DP, bool PAD, bool P16>
@@ -1171,7 +1181,7 @@ extern "C" hipError_t zoo_paged_evict(const zoo::PagedEvictArgs* a, hipStream_t 
     }
   }
   e = hipGetLastError();
-  if (e != hipSuccess || a->most <= 0) return e;
+  if (e != hipSuccess || a->most <= 0 || a->fused) return e;
   // a workgroup for 256 pieces, up to 2^22 of them; more pieces are taken in turn
   const long want = ((long)a->most * a->vec.d + 255) / 256, room = (1 << 22) / rows;
   const int per = (int)(want < room ? want : room > 0 ? room : 1);
