@@ -32,7 +32,7 @@ struct PagedAttnArgs {
   void* o;                   // [B, H * G, D]
   float* logits;             // [B, H * G, pitch] raw products q.k (weights only)
   float* part_o;             // [items, gs, D] partial sums of a split sequence
-  float* part_ml;            // [items, 16, 2] their running maximum (log2 units) and sum
+  float* part_ml;            // [items, wide, 2] their running maximum (log2 units) and sum
   int4* plan;                // [items, 2] who does what, for the join; null where there is none
   long q_b, q_h, table_b;
   PoolStride ks, vs, ss, sos;
@@ -40,9 +40,10 @@ struct PagedAttnArgs {
   int B, H, G, D, pages, cap;
   int pitch;                 // cap rounded up to 16
   int dtype;                 // 0 bf16, 1 fp16, 2 fp32
-  int gs;                    // min(G, 16)
+  int wide;                  // query heads of a workgroup: 16 or 32
+  int gs;                    // min(G, wide)
   int single;                // 1: every sequence is one work item
-  int hbs;                   // blocks of 16 query heads per kv head
+  int hbs;                   // workgroups to the query heads of a kv head
   FastDiv step;              // H * hbs: items from one chunk to the next
   float per_target;          // 0.999 / target: the chunks to aim at over the batch, per head block
   float cached;              // slots of the batch up to which keys and values are left in the caches

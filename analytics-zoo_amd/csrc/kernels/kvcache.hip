@@ -98,7 +98,7 @@ ZOO_DEV float wave_total(float x) {
 #undef ZOO_DPP
 
 struct Work {
-  int b, hk, hb;    // sequence, kv head, block of 16 query heads
+  int b, hk, hb;    // sequence, kv head, block of query heads
   int chunk, n;     // which of the sequence's n chunks
   int s0, s1;       // its slots
   int len;          // the sequence's slots, -1: bad
@@ -307,13 +307,15 @@ ZOO_DEV void gather_weights(const PagedAttnArgs& a, int b, int hk, int s0, int s
 
 // DP: the head width rounded up; PAD: it was rounded; P16: pages of a multiple of 16 rows, so that a
 // 16-slot subtile lies in one page and its address is wave-uniform. Other page sizes look up a page per
-// slot.
-template <int DT, int DP, bool PAD, bool P16>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD ? 2 : 3) void paged_attn_kernel(const PagedAttnArgs a) {
+// slot. NB: blocks of 16 query heads that share what was loaded.
+template <int DT, int DP, bool PAD, bool P16, int NB>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP == 128 && PAD) ? 2 : 3) void paged_attn_kernel(
+    const PagedAttnArgs a) {
   using T = Tile<DT, DP>;
   constexpr int NS = T::NS, KL = T::KL, VC = T::VC, VW = T::VW, VE = T::VE, NA = T::NA, ES = T::ES;
-  extern __shared__ float lds[];  // [4][gb][DP + 4] sums, then [4][16][2] maximum and sum
-  __shared__ float lse[16];
+  constexpr int W = 16 * NB;
+  extern __shared__ float lds[];  // [4][gb][DP + 4] sums, then [4][W][2] maximum and sum
+  __shared__ float lse[W];
   const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6);
   // An unsplit sequence's first page can be looked up before its length is known: the look-up that counts then
   // finds it in the scalar cache.
@@ -326,8 +328,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD
   put_work(a, w, found);
   if (!found) return;
   const int row = lane & 15, quad = lane >> 4;
-  const int gb = min(16, a.G - 16 * w.hb), D = a.D;
-  const int head0 = w.hk * a.G + 16 * w.hb;
+  const int gb = min(W, a.G - W * w.hb), D = a.D;
+  const int head0 = w.hk * a.G + W * w.hb;
   const long out0 = ((long)w.b * a.H * a.G + head0) * D;
   if (w.len <= 0) {
     const float x = w.len < 0 ? __builtin_nanf("") : 0.f;
@@ -337,15 +339,17 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD
   // fp16 cannot hold small weights: they are kept times 2^12 (their maximum is 1, and 16 * 2^12 < 2^16)
   constexpr float kUp = DT == kF16 ? 12.f : 0.f;
 
-  // Q^T: head `row`, the dims that K's loads bring. Heads and dims that are not there are zero.
-  uint4 q[KL];
-  {
-    const char* qp = (const char*)a.q + ((long)w.b * a.q_b + (long)(head0 + min(row, gb - 1)) * a.q_h) * ES;
+  // Q^T: heads row, 16 + row, the dims that K's loads bring. Heads and dims that are not there are zero.
+  uint4 q[NB][KL];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int h = 16 * n + row;
+    const char* qp = (const char*)a.q + ((long)w.b * a.q_b + (long)(head0 + min(h, gb - 1)) * a.q_h) * ES;
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
       const int at = i * 64 + quad * 16;
-      const bool in = row < gb && (!PAD || at < D * ES);
-      q[i] = mask4(*(const uint4*)(qp + (!PAD || at < D * ES ? at : 0)), in);
+      const bool in = h < gb && (!PAD || at < D * ES);
+      q[n][i] = mask4(*(const uint4*)(qp + (!PAD || at < D * ES ? at : 0)), in);
     }
   }
   const int* table = a.table + (long)w.b * a.table_b;
@@ -422,10 +426,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD
     }
   };
 
-  f32x4 acc[NA];
+  f32x4 acc[NB][NA];
+  float m[NB], l[NB];  // of heads 16 n + row; l of this lane's slots only
 #pragma unroll
-  for (int i = 0; i < NA; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;  // of head `row`; l of this lane's slots only
+  for (int n = 0; n < NB; ++n) {
+    m[n] = -INFINITY, l[n] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   float* logit = a.logits ? a.logits + ((long)w.b * a.H * a.G + head0 + row) * a.pitch + 4 * quad : nullptr;
 
   auto stream = [&](auto nt) {
@@ -436,57 +444,64 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD
     }
     for (; base < w.s1; base += T::GRAIN) {
       const bool more = base + T::GRAIN < w.s1, tail = base + T::TS > w.s1;
-      f32x4 s[NS];
+      f32x4 s[NB][NS];
 #pragma unroll
-      for (int u = 0; u < NS; ++u) {
-        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < KL; ++i) {
-          if constexpr (DT == kF32) {
-            s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].x), __uint_as_float(q[i].x), s[u], 0, 0, 0);
-            s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].y), __uint_as_float(q[i].y), s[u], 0, 0, 0);
-            s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].z), __uint_as_float(q[i].z), s[u], 0, 0, 0);
-            s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[u][i].w), __uint_as_float(q[i].w), s[u], 0, 0, 0);
-          } else {
-            s[u] = mma16<DT>(kr[u][i], q[i], s[u]);
+        for (int u = 0; u < NS; ++u) {
+          f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < KL; ++i) {
+            if constexpr (DT == kF32) {
+              const uint4 &k = kr[u][i], &y = q[n][i];
+              x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.x), __uint_as_float(y.x), x, 0, 0, 0);
+              x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.y), __uint_as_float(y.y), x, 0, 0, 0);
+              x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.z), __uint_as_float(y.z), x, 0, 0, 0);
+              x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.w), __uint_as_float(y.w), x, 0, 0, 0);
+            } else {
+              x = mma16<DT>(kr[u][i], q[n][i], x);
+            }
           }
+          s[n][u] = x;
         }
-      }
       if (more) load_k(base + T::GRAIN, nt);
-      if (logit != nullptr && row < gb) {
-        // rows are padded to whole subtiles, so 4 slots go at once
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        if (logit != nullptr && 16 * n + row < gb) {
+          // rows are padded to whole subtiles, so 4 slots go at once
+#pragma unroll
+          for (int u = 0; u < NS; ++u)
+            if (base + 16 * u < w.s1) *(f32x4*)(logit + (long)(16 * n) * a.pitch + base + 16 * u) = s[n][u];
+        }
+        float top = m[n];
 #pragma unroll
         for (int u = 0; u < NS; ++u)
-          if (base + 16 * u < w.s1) *(f32x4*)(logit + base + 16 * u) = s[u];
-      }
-      float top = m;
 #pragma unroll
-      for (int u = 0; u < NS; ++u)
+          for (int r = 0; r < 4; ++r) {
+            s[n][u][r] *= a.c;
+            if (tail && base + 16 * u + 4 * quad + r >= w.s1) s[n][u][r] = -INFINITY;
+            top = fmaxf(top, s[n][u][r]);
+          }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float mu = top == -INFINITY ? 0.f : top;  // nothing but -inf so far: every weight is 0, not NaN
+        const float old = pow2(m[n] - mu);
+        m[n] = top;
+        l[n] *= old;
+        if (__any(old != 1.f)) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[u][r] *= a.c;
-          if (tail && base + 16 * u + 4 * quad + r >= w.s1) s[u][r] = -INFINITY;
-          top = fmaxf(top, s[u][r]);
+          for (int i = 0; i < NA; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[n][i][r] *= old;
         }
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float mu = top == -INFINITY ? 0.f : top;  // nothing but -inf so far: every weight is 0, not NaN
-      const float old = pow2(m - mu);
-      m = top;
-      l *= old;
-      if (__any(old != 1.f)) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i)
+        for (int u = 0; u < NS; ++u)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][r] *= old;
+          for (int r = 0; r < 4; ++r) {
+            s[n][u][r] = pow2(s[n][u][r] - mu + kUp);
+            l[n] += s[n][u][r];
+          }
       }
-#pragma unroll
-      for (int u = 0; u < NS; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[u][r] = pow2(s[u][r] - mu + kUp);
-          l += s[u][r];
-        }
       // a slot behind the last has weight 0, but 0 times what its row happens to hold may be NaN
       if (tail) {
 #pragma unroll
@@ -509,16 +524,21 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD
             for (int c = 0; c < VC; ++c)
 #pragma unroll
               for (int e = 0; e < VE; ++e)
-                acc[c * VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[u][r][c][e]), s[u][r],
-                                                                       acc[c * VE + e], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+                  acc[n][c * VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                      __uint_as_float(vr[u][r][c][e]), s[n][u][r], acc[n][c * VE + e], 0, 0, 0);
       } else {
 #pragma unroll
         for (int u = 0; u < NS; u += 2) {
-          uint4 hi, lo;
-          split2<DT>(s[u][0], s[u][1], hi.x, lo.x);
-          split2<DT>(s[u][2], s[u][3], hi.y, lo.y);
-          split2<DT>(s[u + 1][0], s[u + 1][1], hi.z, lo.z);
-          split2<DT>(s[u + 1][2], s[u + 1][3], hi.w, lo.w);
+          uint4 hi[NB], lo[NB];
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            split2<DT>(s[n][u][0], s[n][u][1], hi[n].x, lo[n].x);
+            split2<DT>(s[n][u][2], s[n][u][3], hi[n].y, lo[n].y);
+            split2<DT>(s[n][u + 1][0], s[n][u + 1][1], hi[n].z, lo[n].z);
+            split2<DT>(s[n][u + 1][2], s[n][u + 1][3], hi[n].w, lo[n].w);
+          }
 #pragma unroll
           for (int c = 0; c < VC; ++c)
 #pragma unroll
@@ -529,8 +549,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD
               x.y = __builtin_amdgcn_perm(vr[u][3][c][e / 2], vr[u][2][c][e / 2], sel);
               x.z = __builtin_amdgcn_perm(vr[u + 1][1][c][e / 2], vr[u + 1][0][c][e / 2], sel);
               x.w = __builtin_amdgcn_perm(vr[u + 1][3][c][e / 2], vr[u + 1][2][c][e / 2], sel);
-              acc[c * VE + e] = mma16<DT>(x, hi, acc[c * VE + e]);
-              acc[c * VE + e] = mma16<DT>(x, lo, acc[c * VE + e]);
+#pragma unroll
+              for (int n = 0; n < NB; ++n) {
+                acc[n][c * VE + e] = mma16<DT>(x, hi[n], acc[n][c * VE + e]);
+                acc[n][c * VE + e] = mma16<DT>(x, lo[n], acc[n][c * VE + e]);
+              }
             }
         }
       }
@@ -541,24 +564,29 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD
     stream(std::bool_constant<P16 && !PAD>{});
   else
     stream(std::false_type{});
-  const bool weights = w.n == 1 && a.logits != nullptr && a.G <= 16;
+  const bool weights = w.n == 1 && a.logits != nullptr && a.G <= W;
   Ahead ahead;
   if (weights && threadIdx.x < w.s1) ahead = weights_ahead(a, w.b, w.hk, threadIdx.x, w.s1);
   // the four waves' sums meet in LDS
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
-  if (__any(bad)) l = __builtin_nanf("");
   constexpr int LD = DP + 4;
   float* ml = lds + 4 * gb * LD;
-  if (row < gb) {
+  const bool wrong = __any(bad);
 #pragma unroll
-    for (int i = 0; i < NA; ++i)
+  for (int n = 0; n < NB; ++n) {
+    l[n] += __shfl_xor(l[n], 16, 64);
+    l[n] += __shfl_xor(l[n], 32, 64);
+    if (wrong) l[n] = __builtin_nanf("");
+    const int h = 16 * n + row;
+    if (h < gb) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        lds[(wave * gb + row) * LD + (i / VE) * (16 * VE) + (quad * 4 + r) * VE + i % VE] = acc[i][r];
-    if (quad == 0) {
-      ml[(wave * 16 + row) * 2] = m;
-      ml[(wave * 16 + row) * 2 + 1] = l;
+      for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          lds[(wave * gb + h) * LD + (i / VE) * (16 * VE) + (quad * 4 + r) * VE + i % VE] = acc[n][i][r];
+      if (quad == 0) {
+        ml[(wave * W + h) * 2] = m[n];
+        ml[(wave * W + h) * 2 + 1] = l[n];
+      }
     }
   }
   __syncthreads();
@@ -566,13 +594,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD
     const int g = i / DP, d = i & (DP - 1);
     float top = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) top = fmaxf(top, ml[(x * 16 + g) * 2]);
+    for (int x = 0; x < 4; ++x) top = fmaxf(top, ml[(x * W + g) * 2]);
     const float mu = top == -INFINITY ? 0.f : top;
     float sum = 0.f, o = 0.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const float f = pow2(ml[(x * 16 + g) * 2] - mu);
-      sum += f * ml[(x * 16 + g) * 2 + 1];
+      const float f = pow2(ml[(x * W + g) * 2] - mu);
+      sum += f * ml[(x * W + g) * 2 + 1];
       o += f * lds[(x * gb + g) * LD + d];
     }
     if (!PAD || d < D) {
@@ -583,8 +611,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : DT == kF32 && DP == 128 && PAD
     }
     if (d == 0) {
       if (a.part_ml != nullptr) {
-        a.part_ml[((long)item_of(a) * 16 + g) * 2] = top;
-        a.part_ml[((long)item_of(a) * 16 + g) * 2 + 1] = sum;
+        a.part_ml[((long)item_of(a) * W + g) * 2] = top;
+        a.part_ml[((long)item_of(a) * W + g) * 2 + 1] = sum;
       }
       lse[g] = top + log2f(sum) - kUp;
     }
@@ -614,20 +642,21 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Pag
   Work w;
   if (!get_work(a, w)) return;
   // an unsplit sequence is ready but for the weights of kv heads with more than one block of query heads
-  const bool weights = a.logits != nullptr && w.hb == 0 && (w.n > 1 || a.G > 16);
+  const bool weights = a.logits != nullptr && w.hb == 0 && (w.n > 1 || a.hbs > 1);
   if (w.len <= 0 || (w.n == 1 && !weights)) return;
   const int tid = threadIdx.x;
+  const long next = (long)a.step.d * a.wide * 2;   // from one chunk's maxima and sums to the next one's
   Ahead ahead;
   if (weights) {
     if (w.s0 + tid < w.s1) ahead = weights_ahead(a, w.b, w.hk, w.s0 + tid, w.s1);
     // log2 of the sum of exponentials of all heads, 16 threads to a head
     for (int g0 = 0; g0 < a.G; g0 += kJoinThreads / 16) {
       const int g = g0 + (tid >> 4);
-      const float* ml = a.part_ml + ((long)(w.first + (g >> 4)) * 16 + (g & 15)) * 2;
+      const float* ml = a.part_ml + ((long)(w.first + g / a.wide) * a.wide + g % a.wide) * 2;
       float m = -INFINITY, l = 0.f, x = 0.f;
       if (g < a.G) {
 #pragma unroll 4
-        for (int i = tid & 15; i < w.n; i += 16) merge(m, l, x, ml[i * (long)a.step.d * 32], ml[i * (long)a.step.d * 32 + 1], 0.f);
+        for (int i = tid & 15; i < w.n; i += 16) merge(m, l, x, ml[i * next], ml[i * next + 1], 0.f);
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) merge(m, l, x, __shfl_xor(m, o, 64), __shfl_xor(l, o, 64), 0.f);
@@ -636,16 +665,16 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Pag
     if (w.n == 1) __syncthreads();
   }
   if (w.n > 1) {
-    const int E = min(16, a.G - 16 * w.hb) * a.D;
+    const int E = min(a.wide, a.G - a.wide * w.hb) * a.D;
     const int per = ((E + w.n - 1) / w.n + 15) & ~15;
     const int e0 = w.chunk * per, e1 = min(E, e0 + per);
     int wide = 16;
     while (wide < per && wide < kJoinThreads) wide *= 2;
     const int ways = kJoinThreads / wide, who = tid / wide;
     const float* po = a.part_o + (long)w.first * a.gs * a.D;
-    const float* ml = a.part_ml + (long)w.first * 32;
-    const long step_o = (long)a.step.d * a.gs * a.D, step_m = (long)a.step.d * 32;
-    const long out0 = ((long)w.b * a.H * a.G + w.hk * a.G + 16 * w.hb) * a.D;
+    const float* ml = a.part_ml + (long)w.first * a.wide * 2;
+    const long step_o = (long)a.step.d * a.gs * a.D;
+    const long out0 = ((long)w.b * a.H * a.G + w.hk * a.G + a.wide * w.hb) * a.D;
     if (e0 >= e1) __syncthreads();
     for (int e = e0; e < e1; e += wide) {
       const int at = e + (tid & (wide - 1));
@@ -654,7 +683,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Pag
         const int g = at / a.D;
 #pragma unroll 4
         for (int i = who; i < w.n; i += ways)
-          merge(m, l, x, ml[i * step_m + g * 2], ml[i * step_m + g * 2 + 1], po[i * step_o + at]);
+          merge(m, l, x, ml[i * next + g * 2], ml[i * next + g * 2 + 1], po[i * step_o + at]);
       }
       // threads of a wave with the same element first: lanes that are `wide` apart
       for (int o = wide; o < 64; o *= 2) merge(m, l, x, __shfl_xor(m, o, 64), __shfl_xor(l, o, 64), __shfl_xor(x, o, 64));
@@ -1106,36 +1135,41 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(const PagedEvictA
   move_rows(a, row, r, a.count[r], (blockIdx.x - r * blocks_per_row) * 256 + threadIdx.x, blocks_per_row * 256);
 }
 
-template <int DT, int DP, bool PAD, bool P16>
+template <int DT, int DP, bool PAD, bool P16, int NB>
 hipError_t attn_launch(const PagedAttnArgs& a, int items, hipStream_t st) {
-  const int gb = a.G < 16 ? a.G : 16;
-  const size_t lds = (size_t)(4 * gb * (DP + 4) + 128) * sizeof(float);
+  const size_t lds = (size_t)(4 * a.gs * (DP + 4) + 4 * 16 * NB * 2) * sizeof(float);
   if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute((const void*)paged_attn_kernel<DT, DP, PAD, P16>,
+    const hipError_t e = hipFuncSetAttribute((const void*)paged_attn_kernel<DT, DP, PAD, P16, NB>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  paged_attn_kernel<DT, DP, PAD, P16><<<items, 256, lds, st>>>(a);
+  paged_attn_kernel<DT, DP, PAD, P16, NB><<<items, 256, lds, st>>>(a);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && (!a.single || (a.logits != nullptr && a.G > 16))) {
+  if (e == hipSuccess && (!a.single || (a.logits != nullptr && a.hbs > 1))) {
     paged_attn_join_kernel<<<items, kJoinThreads, 0, st>>>(a);
     e = hipGetLastError();
   }
   return e;
 }
 
-template <int DT, int DP>
+template <int DT, int DP, int NB>
 hipError_t attn_pick(const PagedAttnArgs& a, int items, hipStream_t st) {
   const bool p16 = a.page.d % 16 == 0;
-  if (a.D == DP) return p16 ? attn_launch<DT, DP, false, true>(a, items, st) : attn_launch<DT, DP, false, false>(a, items, st);
-  return p16 ? attn_launch<DT, DP, true, true>(a, items, st) : attn_launch<DT, DP, true, false>(a, items, st);
+  if (a.D == DP) return p16 ? attn_launch<DT, DP, false, true, NB>(a, items, st) : attn_launch<DT, DP, false, false, NB>(a, items, st);
+  return p16 ? attn_launch<DT, DP, true, true, NB>(a, items, st) : attn_launch<DT, DP, true, false, NB>(a, items, st);
+}
+
+template <int DT, int NB>
+hipError_t attn_width(const PagedAttnArgs& a, int items, hipStream_t st) {
+  if (a.D <= 64) return attn_pick<DT, 64, NB>(a, items, st);
+  if (a.D <= 128) return attn_pick<DT, 128, NB>(a, items, st);
+  // 32 heads of 256 dims in 32 bits do not fit the registers: the bindings never ask for them
+  return attn_pick<DT, 256, DT == kF32 ? 1 : NB>(a, items, st);
 }
 
 template <int DT>
 hipError_t attn_dims(const PagedAttnArgs& a, int items, hipStream_t st) {
-  if (a.D <= 64) return attn_pick<DT, 64>(a, items, st);
-  if (a.D <= 128) return attn_pick<DT, 128>(a, items, st);
-  return attn_pick<DT, 256>(a, items, st);
+  return a.wide == 16 ? attn_width<DT, 1>(a, items, st) : attn_width<DT, 2>(a, items, st);
 }
 
 }  // namespace

@@ -3195,7 +3195,8 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   req_rows(q, "q");
   TORCH_CHECK(q.size(1) >= c.H && q.size(1) % c.H == 0, what, ": the heads of q must be a multiple of the cache's kv heads");
   TORCH_CHECK(std::isfinite(scale), what, ": scale must be finite");
-  const int64_t G = q.size(1) / c.H, hbs = (G + 15) / 16;
+  const int64_t G = q.size(1) / c.H;
+  const int64_t wide = G > 16 && (c.dtype != 2 || c.D <= 128) ? 32 : 16, hbs = (G + wide - 1) / wide;
   TORCH_CHECK(G <= zoo::kKvMaxGroup, what, ": at most 256 query heads may share a kv head");
   const bool weights = scores.has_value() && scores->defined();
   TORCH_CHECK(weights || !scores_out.has_value(), what, ": scores_out without scores");
@@ -3221,9 +3222,9 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   auto f32 = q.options().dtype(at::kFloat);
   torch::Tensor ml, po, logits, plan;
   const int64_t pitch = (c.cap + 15) / 16 * 16;
-  const int64_t gs = std::min<int64_t>(G, 16);
-  if (!a.single || (weights && G > 16)) {
-    ml = torch::empty({items, 16, 2}, f32);
+  const int64_t gs = std::min<int64_t>(G, wide);
+  if (!a.single || (weights && hbs > 1)) {
+    ml = torch::empty({items, wide, 2}, f32);
     plan = torch::empty({items, 8}, lengths.options());
     a.plan = reinterpret_cast<int4*>(plan.data_ptr<int>());
   }
@@ -3243,7 +3244,7 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   a.ks = pool_stride(kp), a.vs = pool_stride(vp);
   a.page = fast_div((uint32_t)c.page);
   a.B = c.B, a.H = c.H, a.G = G, a.D = c.D, a.pages = c.P, a.cap = c.cap, a.pitch = pitch, a.dtype = c.dtype, a.gs = gs;
-  a.hbs = hbs, a.step = fast_div((uint32_t)per_seq);
+  a.wide = wide, a.hbs = hbs, a.step = fast_div((uint32_t)per_seq);
   // Past 400 MB the caches (256 MB) hold nothing until the next token, and loads that go past them are faster: 537 MB
   // 89 us, 101 through them; 4.3 GB 636 and 713. Below, they are slower: 314 MB 84 and 81, 50 MB 14.5 and 12.2. Kv heads
   // with several blocks of query heads read everything several times: 537 MB twice 188 us, through the caches 130.

@@ -100,6 +100,13 @@ CASES = [
     (1, 24, 64, 48, HF, "phsd", [900, 20]),          # two blocks of query heads
     (2, 71, 64, 16, BF, "phsd", [100, 300]),         # five of them
     (1, 2, 16, 24, BF, "phsd", [500, 3]),
+    (2, 17, 128, 64, BF, "phsd", [700, 1, 0]),
+    (1, 32, 256, 16, HF, "phsd", [600, 33]),
+    (1, 40, 200, 16, FL, "phsd", [300, 15]),
+    (1, 33, 96, 32, BF, "pshd", [1200, 64]),
+    (1, 32, 72, 11, FL, "phsd", [900, 12]),
+    (1, 256, 64, 16, BF, "phsd", [2100, 40]),
+    (2, 24, 24, 16, HF, "phsd", [2600, 40, 700]),
     (2, 1, 40, 7, BF, "phsd", [400, 0, 6, 7, 8]),    # no multiple of 16 in sight
     (2, 5, 80, 1, HF, "phsd", [270, 4]),
     (3, 2, 96, 100, FL, "pshd", [410, 99, 100, 101]),
@@ -134,7 +141,7 @@ def _check_attention(dev, H, G, D, page, dtype, order, lengths, weights):
 
 
 @pytest.mark.parametrize("weights", [False, True])
-@pytest.mark.parametrize("H,G,D,page,dtype,order,lengths", CASES[:14])
+@pytest.mark.parametrize("H,G,D,page,dtype,order,lengths", CASES[:16])
 def test_attention_cpu(H, G, D, page, dtype, order, lengths, weights):
     _check_attention("cpu", H, G, D, page, dtype, order, lengths, weights)
 
