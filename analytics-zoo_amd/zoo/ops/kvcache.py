@@ -49,8 +49,9 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, scores
 
     With ``scores``, every slot in use gathers the weight that the query heads of its kv head gave it:
     ``scores_out[slot] = scores[slot] + sum(weights)``; ``scores_out`` defaults to ``scores`` itself. This takes
-    ``batch * heads * capacity`` floats of workspace, where the capacity is what a row of the table can name, or
-    ``max_length`` if that is given: no sequence is longer."""
+    ``batch * heads * capacity`` floats of workspace, where the capacity is what a row of the table can name: pass a
+    narrower view of a wide table, or ``max_length``, a bound on the lengths (a sequence that is longer comes out
+    NaN)."""
     _no_grad("paged_attention", q, k_pages, v_pages, scores)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
@@ -167,17 +168,23 @@ class PagedKVCache:
             self.lengths[r] = 0
             self.seen[r] = 0
 
+    def _table(self):
+        # no wider than the pages in hand, which bounds the operators' workspace
+        return self.page_table[:, :max(1, max(len(own) for own in self._pages))]
+
     def append(self, i, k, v, counts=None, rows=None):
-        """``paged_append`` to layer ``i``; returns the new lengths, which :meth:`advance` makes the cache's."""
+        """``paged_append`` to layer ``i`` of all rows, or of the ``rows`` (int64 [n] on the device); returns the new
+        lengths, which :meth:`advance` makes the cache's."""
         kp, vp, scores, positions = self.layer(i)
         at = slice(None) if rows is None else rows
-        return paged_append(k, v, kp, vp, self.page_table[at], self.lengths[at], counts=counts, seen=self.seen[at],
+        return paged_append(k, v, kp, vp, self._table()[at], self.lengths[at], counts=counts, seen=self.seen[at],
                             scores=scores, positions=positions)
 
-    def attend(self, i, q, lengths, scale=None):
-        """``paged_attention`` over layer ``i`` of all rows, gathering weights if there is a budget."""
+    def attend(self, i, q, lengths, scale=None, rows=None):
+        """``paged_attention`` over layer ``i``, gathering weights if there is a budget."""
         kp, vp, scores, _ = self.layer(i)
-        return paged_attention(q, kp, vp, self.page_table, lengths, scale=scale, scores=scores)
+        at = slice(None) if rows is None else rows
+        return paged_attention(q, kp, vp, self._table()[at], lengths, scale=scale, scores=scores)
 
     def advance(self, tokens, lengths, rows=None, evict=True):
         """Ends a step that gave the rows ``tokens`` tokens (a number, or one for each row): ``lengths`` are in use now,
@@ -200,7 +207,7 @@ class PagedKVCache:
         that a sequence of budget + slack + 1 slots does not need."""
         if self.budget is None or max(self._slots) <= self.budget + self.slack:
             return
-        new = paged_evict(self.k, self.v, self.scores, self.positions, self.page_table, self.lengths, self.seen,
+        new = paged_evict(self.k, self.v, self.scores, self.positions, self._table(), self.lengths, self.seen,
                           self.budget, self.recent)
         self.lengths.copy_(new)
         self._slots = [min(n, self.budget) for n in self._slots]

@@ -220,20 +220,22 @@ class TransformerLayer(Layer):
         return x
 
     @torch.no_grad()
-    def decode(self, xs, cache):
-        """One token of every row of ``cache``: ``xs`` = [token_ids, position_ids] ([batch]). Returns the sequence
-        output of these tokens [batch, hidden]."""
-        if xs[0].dim() != 1 or xs[0].shape[0] != cache.batch:
+    def decode(self, xs, cache, rows=None):
+        """One token of every row of ``cache``, or of the rows ``rows`` (a list of numbers): ``xs`` = [token_ids,
+        position_ids] ([n]). Returns the sequence output of these tokens [n, hidden]."""
+        n = cache.batch if rows is None else len(rows)
+        if xs[0].dim() != 1 or xs[0].shape[0] != n or (rows is not None and len(set(rows)) != n):
             raise ValueError("decode: one token for each row of the cache")
-        cache.reserve(1)
+        cache.reserve(1, rows)
+        sub = None if rows is None else torch.tensor(list(rows)).to(cache.k.device)
         new = []
 
         def cached(i, blk, qkv):
             q, k, v = self._split(qkv, blk, cache)
-            new[:] = [cache.append(i, k, v)]
-            return cache.attend(i, q[:, 0], new[0]).reshape(qkv.shape[0], 1, -1).to(qkv.dtype)
+            new[:] = [cache.append(i, k, v, rows=sub)]
+            return cache.attend(i, q[:, 0], new[0], rows=sub).reshape(n, 1, -1).to(qkv.dtype)
         x = self._cached_run(self._embed([t.unsqueeze(1) for t in xs]), cached)
-        cache.advance(1, new[0])
+        cache.advance(1, new[0], rows)
         return x[:, 0]
 
 

@@ -83,6 +83,14 @@ def test_padded_prompts_and_rows_that_come_and_go(dev):
     with torch.no_grad():
         near(got[0], t([torch.cat([tok[0], nxt[:1], nxt[:1]])[None], torch.cat([pos[0], npos[:1], npos[:1] + 1])[None]])[0][0, -1], dev)
         near(got[2], t([torch.cat([tok2[0], nxt[2:3]])[None], torch.cat([pos2[0], npos[2:3] + 1])[None]])[0][0, -1], dev)
+    # some rows take a step, the others wait
+    before = got
+    got = t.decode([nxt[1:3], npos[1:3] + 2], cache, rows=[1, 2])
+    assert cache.lengths.tolist() == [32, 4, 14, 2] and cache.seen.tolist() == [32, 4, 14, 2]
+    with torch.no_grad():
+        near(got[1], t([torch.cat([tok2[0], nxt[2:3], nxt[2:3]])[None],
+                        torch.cat([pos2[0], npos[2:3] + 1, npos[2:3] + 2])[None]])[0][0, -1], dev)
+    assert torch.isfinite(before.float()).all()
     # the book: no page in two rows
     used = [p for own in cache._pages for p in own]
     assert len(used) == len(set(used)) and not set(used) & set(cache._free) and len(used) + len(cache._free) == 14
@@ -137,6 +145,8 @@ def test_refusals():
         t.decode([tok[:, 0], pos[:, 0]], cache)
     with pytest.raises(ValueError):
         t.decode([tok, pos], cache)
+    with pytest.raises(ValueError):
+        t.decode([tok[:, 0], pos[:, 0]], cache, rows=[1, 1])
     with pytest.raises(ValueError):
         t.prefill([tok, pos], cache, rows=[0])
     with pytest.raises(ValueError):
@@ -244,3 +254,46 @@ def test_the_book_on_its_own():
         c.reserve(21)
     with pytest.raises(RuntimeError):
         c.replayed(5)
+
+
+@pytest.mark.gpu
+def test_captured_operators_over_long_rows(gpu):
+    """Split attention with gathered weights and an eviction that shares out its rows, captured together and replayed
+    with other work in between, against eager calls."""
+    from test_kvcache import make
+    lengths = [18000, 5, 0, 17001]
+    q, k, v, table, n = make(4, 2, 4, 64, 128, lengths, torch.bfloat16, "cuda")
+    g = torch.Generator("cuda").manual_seed(2)
+    scores = torch.rand(k.shape[:3], generator=g, device="cuda")
+    positions = torch.randint(0, 18000, k.shape[:3], generator=g, device="cuda", dtype=torch.int32)
+    seen = n + 3
+
+    def step(q, k, v, scores, positions):
+        o = paged_attention(q, k, v, table, n, scores=scores)
+        return o, paged_evict(k, v, scores, positions, table, n, seen, 9000, 500)
+
+    start = [t.clone() for t in (k, v, scores, positions)]
+    pools = [t.clone() for t in start]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(q, *pools)
+    torch.cuda.current_stream().wait_stream(side)
+    x = q.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, new = step(x, *pools)
+    for i in range(5):
+        fresh = q * (0.5 + 0.25 * i)
+        for a, b in zip(pools, start):
+            a.copy_(b)
+        x.copy_(fresh)
+        graph.replay()
+        junk = torch.randn(1024, 1024, device="cuda").sum()
+        eager = [t.clone() for t in start]
+        want, want_n = step(fresh, *eager)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(new, want_n) and want_n.tolist() == [9000, 5, 0, 9000]
+        for a, b in zip(pools, eager):
+            assert torch.equal(a.nan_to_num() if a.is_floating_point() else a, b.nan_to_num() if b.is_floating_point() else b)
+    assert torch.isfinite(junk)
