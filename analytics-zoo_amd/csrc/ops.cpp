@@ -3124,6 +3124,12 @@ void req_rows(const torch::Tensor& t, const char* what) {
     TORCH_CHECK(t.size(i) <= 1 || t.stride(i) % n == 0, what, ": rows must start on 16 bytes");
 }
 
+void paged_no_grad(std::initializer_list<const torch::Tensor*> ts, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const torch::Tensor* t : ts)
+    TORCH_CHECK(!t->requires_grad(), what, " has no backward pass: call it under torch.no_grad()");
+}
+
 // slots that a row of the table may name (at most max_length of them, if that is given)
 PagedCache paged_check(const torch::Tensor& kp, const torch::Tensor& vp, const torch::Tensor& table,
                        const torch::Tensor& lengths, c10::optional<int64_t> max_length, const char* what) {
@@ -3188,6 +3194,7 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
                               c10::optional<torch::Tensor> scores_out, c10::optional<int64_t> max_length) {
   const char* what = "paged_attention";
   const PagedCache c = paged_check(kp, vp, table, lengths, max_length, what);
+  paged_no_grad({&q, &kp, &vp}, what);
   c10::DeviceGuard guard(kp.device());
   TORCH_CHECK(q.dim() == 3 && q.size(0) == c.B && q.size(2) == c.D && q.scalar_type() == kp.scalar_type() &&
                   q.device() == kp.device(),
@@ -3202,6 +3209,7 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   TORCH_CHECK(weights || !scores_out.has_value(), what, ": scores_out without scores");
   if (weights) {
     paged_side(*scores, kp, at::kFloat, "scores", what);
+    paged_no_grad({&*scores}, what);
     if (!scores_out.has_value()) scores_out = scores;
     paged_side(*scores_out, kp, at::kFloat, "scores_out", what);
     at::assert_no_internal_overlap(*scores_out);
@@ -3260,6 +3268,7 @@ torch::Tensor paged_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, t
                            c10::optional<torch::Tensor> scores, c10::optional<torch::Tensor> positions) {
   const char* what = "paged_append";
   const PagedCache c = paged_check(kp, vp, table, lengths, c10::nullopt, what);
+  paged_no_grad({&k, &v, &kp, &vp}, what);
   c10::DeviceGuard guard(kp.device());
   for (const torch::Tensor* t : {&k, &v}) {
     TORCH_CHECK(t->dim() == 4 && t->size(0) == c.B && t->size(2) == c.H && t->size(3) == c.D &&
@@ -3306,6 +3315,7 @@ torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scor
                           torch::Tensor scores_out, torch::Tensor positions_out) {
   const char* what = "paged_evict";
   const PagedCache c = paged_check(kp, vp, table, lengths, c10::nullopt, what);
+  paged_no_grad({&kp, &vp, &scores}, what);
   c10::DeviceGuard guard(kp.device());
   TORCH_CHECK(budget >= 1 && budget <= zoo::kKvMaxSlots, what, ": budget must be from 1 to 2^30");
   TORCH_CHECK(recent >= 0 && recent <= budget, what, ": recent must be from 0 to the budget");

@@ -52,11 +52,11 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, scores
     ``batch * heads * capacity`` floats of workspace, where the capacity is what a row of the table can name: pass a
     narrower view of a wide table, or ``max_length``, a bound on the lengths (a sequence that is longer comes out
     NaN)."""
-    _no_grad("paged_attention", q, k_pages, v_pages, scores)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if k_pages.is_cuda:
         return native().paged_attention(q, k_pages, v_pages, page_table, lengths, scale, scores, scores_out, max_length)
+    _no_grad("paged_attention", q, k_pages, v_pages, scores)
     return _attention_ref(q, k_pages, v_pages, page_table, lengths, scale, scores, scores_out, max_length)
 
 
@@ -67,9 +67,9 @@ def paged_append(k, v, k_pages, v_pages, page_table, lengths, counts=None, seen=
     ``seen[b] + t`` (``seen``: int32 [batch], the tokens each sequence has had; ``lengths`` by default). Returns the
     new lengths as a new tensor. Tokens that the table has no room for are not written, but counted: the
     sequence is then longer than its table and its attention NaN."""
-    _no_grad("paged_append", k, v, k_pages, v_pages)
     if k_pages.is_cuda:
         return native().paged_append(k, v, k_pages, v_pages, page_table, lengths, counts, seen, scores, positions)
+    _no_grad("paged_append", k, v, k_pages, v_pages)
     return _append_ref(k, v, k_pages, v_pages, page_table, lengths, counts, seen, scores, positions)
 
 
@@ -82,12 +82,12 @@ def paged_evict(k_pages, v_pages, scores, positions, page_table, lengths, seen, 
     position, so no more rows move than have to. Returns the new lengths ``min(lengths, budget)`` as a new tensor.
 
     Scores and positions of the kept slots go to ``scores_out`` and ``positions_out``, by default where they were."""
-    _no_grad("paged_evict", k_pages, v_pages, scores)
     scores_out = scores if scores_out is None else scores_out
     positions_out = positions if positions_out is None else positions_out
     if k_pages.is_cuda:
         return native().paged_evict(k_pages, v_pages, scores, positions, page_table, lengths, seen, budget, recent,
                                     scores_out, positions_out)
+    _no_grad("paged_evict", k_pages, v_pages, scores)
     return _evict_ref(k_pages, v_pages, scores, positions, page_table, lengths, seen, budget, recent, scores_out,
                       positions_out)
 

@@ -413,6 +413,9 @@ def test_refusals(dev):
     no(paged_attention, q, k, v, table, n, scores_out=s)
     no(paged_attention, q, k, v, table, n, max_length=-1)
     no(paged_attention, q.float().requires_grad_(), k.float(), v.float(), table, n)
+    no(paged_attention, q, k, v, table, n, scores=s.clone().requires_grad_())
+    no(paged_append, x.clone().requires_grad_(), x, k, v, table, n)
+    no(paged_evict, k, v, s.clone().requires_grad_(), p, table, n, n, 4)
     no(paged_append, x[:1], x[:1], k, v, table, n)
     no(paged_append, x[..., :8], x[..., :8], k, v, table, n)
     no(paged_append, x.float(), x.float(), k, v, table, n)
