@@ -43,6 +43,7 @@ struct PagedAttnArgs {
   int wide;                  // query heads of a workgroup: 16 or 32
   int gs;                    // min(G, wide)
   int single;                // 1: every sequence is one work item
+  int held;                  // 1: no `logits`, an unsplit sequence's products stay in LDS
   int hbs;                   // workgroups to the query heads of a kv head
   FastDiv step;              // H * hbs: items from one chunk to the next
   float per_target;          // 0.999 / target: the chunks to aim at over the batch, per head block

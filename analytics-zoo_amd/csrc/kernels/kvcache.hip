@@ -270,6 +270,10 @@ struct Ahead {
   float was[kWays];
 };
 
+ZOO_DEV const float* logits_of(const PagedAttnArgs& a, int b, int hk) {
+  return a.logits + ((long)b * a.H + hk) * a.G * a.pitch;
+}
+
 ZOO_DEV Ahead weights_ahead(const PagedAttnArgs& a, int b, int hk, int s, int s1) {
   const int* table = a.table + (long)b * a.table_b;
   const float* in = a.scores + (long)hk * a.ss.head;
@@ -285,9 +289,10 @@ ZOO_DEV Ahead weights_ahead(const PagedAttnArgs& a, int b, int hk, int s, int s1
   return x;
 }
 
-ZOO_DEV void gather_weights(const PagedAttnArgs& a, int b, int hk, int s0, int s1, Ahead x, const float* lse) {
+// `logit`: of the kv head's first query head, in memory or in LDS
+ZOO_DEV void gather_weights(const PagedAttnArgs& a, int b, int hk, int s0, int s1, Ahead x, const float* lse,
+                            const float* logit) {
   const int G = a.G, step = blockDim.x;
-  const float* logit = a.logits + ((long)b * a.H + hk) * G * a.pitch;
   float* out = a.scores_out + (long)hk * a.sos.head;
   for (int s = s0 + threadIdx.x; s < s1; s += kWays * step) {
     float sum[kWays];
@@ -440,6 +445,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
     for (int i = 0; i < NA; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   float* logit = a.logits ? a.logits + ((long)w.b * a.H * a.G + head0 + row) * a.pitch + 4 * quad : nullptr;
+  float* held = lds + 4 * gb * (DP + 4) + 8 * W;   // [gb][pitch] where the products fit
 
   auto stream = [&](auto nt) {
     int base = w.s0 + wave * T::TS;
@@ -472,6 +478,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
       if (more) load_k(base + T::GRAIN, nt);
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
+        if (a.held && 16 * n + row < gb) {
+#pragma unroll
+          for (int u = 0; u < NS; ++u)
+            if (base + 16 * u < w.s1) *(f32x4*)(held + (16 * n + row) * a.pitch + base + 16 * u + 4 * quad) = s[n][u];
+        }
         if (logit != nullptr && 16 * n + row < gb) {
           // rows are padded to whole subtiles, so 4 slots go at once
 #pragma unroll
@@ -569,7 +580,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
     stream(std::bool_constant<P16 && !PAD>{});
   else
     stream(std::false_type{});
-  const bool weights = w.n == 1 && a.logits != nullptr && a.G <= W;
+  const bool weights = a.held || (w.n == 1 && a.logits != nullptr && a.G <= W);
   Ahead ahead;
   if (weights && threadIdx.x < w.s1) ahead = weights_ahead(a, w.b, w.hk, threadIdx.x, w.s1);
   // the four waves' sums meet in LDS
@@ -624,7 +635,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
   }
   if (weights) {
     __syncthreads();    // orders the waves' products, which this workgroup reads back, as well
-    gather_weights(a, w.b, w.hk, 0, w.s1, ahead, lse);
+    if (a.held)
+      gather_weights(a, w.b, w.hk, 0, w.s1, ahead, lse, held);
+    else
+      gather_weights(a, w.b, w.hk, 0, w.s1, ahead, lse, logits_of(a, w.b, w.hk));
   }
 }
 
@@ -702,7 +716,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Pag
       __syncthreads();
     }
   }
-  if (weights) gather_weights(a, w.b, w.hk, w.s0, w.s1, ahead, lse);
+  if (weights) gather_weights(a, w.b, w.hk, w.s0, w.s1, ahead, lse, logits_of(a, w.b, w.hk));
 }
 
 // ---- append: one thread moves 16 bytes of a token's key row and of its value row ----
@@ -1147,7 +1161,7 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(const PagedEvictA
 
 template <int DT, int DP, bool PAD, bool P16, int NB>
 hipError_t attn_launch(const PagedAttnArgs& a, int items, hipStream_t st) {
-  const size_t lds = (size_t)(4 * a.gs * (DP + 4) + 4 * 16 * NB * 2) * sizeof(float);
+  const size_t lds = (size_t)(4 * a.gs * (DP + 4) + 4 * 16 * NB * 2 + (a.held ? a.gs * a.pitch : 0)) * sizeof(float);
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void*)paged_attn_kernel<DT, DP, PAD, P16, NB>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

@@ -3237,14 +3237,16 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
     a.plan = reinterpret_cast<int4*>(plan.data_ptr<int>());
   }
   if (!a.single) po = torch::empty({items, gs, c.D}, f32);
-  if (weights) logits = torch::empty({c.B, c.H * G, pitch}, f32);
+  // 16 KB of products leave room for three workgroups to a CU
+  a.held = weights && a.single && hbs == 1 && gs * pitch <= 4096;
+  if (weights && !a.held) logits = torch::empty({c.B, c.H * G, pitch}, f32);
   a.q = q.data_ptr(), a.k = kp.data_ptr(), a.v = vp.data_ptr();
   a.table = table.data_ptr<int>(), a.len = lengths.data_ptr<int>();
   a.o = o.data_ptr();
   if (weights) {
     a.scores = scores->data_ptr<float>(), a.scores_out = scores_out->data_ptr<float>();
     a.ss = pool_stride(*scores), a.sos = pool_stride(*scores_out);
-    a.logits = logits.data_ptr<float>();
+    a.logits = a.held ? nullptr : logits.data_ptr<float>();
   }
   a.part_ml = ml.defined() ? ml.data_ptr<float>() : nullptr;
   a.part_o = po.defined() ? po.data_ptr<float>() : nullptr;
