@@ -48,6 +48,7 @@ struct PagedAttnArgs {
   FastDiv step;              // H * hbs: items from one chunk to the next
   float per_target;          // 0.999 / target: the chunks to aim at over the batch, per head block
   float cached;              // slots of the batch up to which keys and values are left in the caches
+  int big;                   // whether there can be more, for sequences of one work item each
   int at_once;               // chunks per head block that the chip can run at once, 0: fewer than B
   float c;                   // scale * log2(e)
 };

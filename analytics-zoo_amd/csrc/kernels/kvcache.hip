@@ -118,9 +118,6 @@ ZOO_DEV int chunk_size(float want, int grain) {
   return max((int)ceilf(fminf(want, 0x1p30f) / grain), 1) * grain;
 }
 
-// Cuts the batch into chunks of `size` slots, a multiple of `grain`, such that there are at most
-// target (1 + 1 / 512) + B of them per head block, and finds the chunk of this workgroup; every wave does so alone.
-// Every sequence has a chunk, if an empty one. False for the items that are not needed.
 // The logical item of this workgroup. Blocks of query heads of one kv head read the same keys and values: they are
 // put 8 workgroups apart, on one XCD, so that its L2 serves all but the first (there are 8 XCDs, and
 // workgroups go to them in turn).
@@ -131,6 +128,9 @@ ZOO_DEV int item_of(const PagedAttnArgs& a) {
   return (g + 1) * group <= (int)gridDim.x ? g * group + (in & 7) * a.hbs + (in >> 3) : x;
 }
 
+// Cuts the batch into chunks of `size` slots, a multiple of `grain`, such that there are at most
+// target (1 + 1 / 512) + B of them per head block, and finds the chunk of this workgroup; every wave does so alone.
+// Every sequence has a chunk, if an empty one. False for the items that are not needed.
 ZOO_DEV bool find_work(const PagedAttnArgs& a, int grain, Work& w) {
   const int lane = threadIdx.x & 63;
   const int item = item_of(a);
@@ -138,7 +138,7 @@ ZOO_DEV bool find_work(const PagedAttnArgs& a, int grain, Work& w) {
   w.hb = 0, w.hk = hh;
   if (a.hbs > 1) w.hk = hh / a.hbs, w.hb = hh - w.hk * a.hbs;
   if (a.single) {
-    w.b = uni(t), w.chunk = 0, w.n = 1, w.first = item, w.big = false;
+    w.b = uni(t), w.chunk = 0, w.n = 1, w.first = item, w.big = a.big;
     w.len = seq_len(a.len, w.b, a.cap);
     w.s0 = 0, w.s1 = w.len;
     return true;
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
   int early = 0;
   if (P16 && a.single && a.cap > 0)
     early = fixed(a.table + (long)fdiv(item_of(a), a.step) * a.table_b)[fdiv(min(wave * T::TS, a.cap - 1), a.page)];
-  Work w;
+  Work w{};
   const bool found = find_work(a, T::GRAIN, w);
   asm volatile("" ::"s"(early));   // keeps the look-up
   put_work(a, w, found);
@@ -1167,7 +1167,7 @@ __global__ __launch_bounds__(256) void paged_evict_move_kernel(const PagedEvictA
 template <int DT, int DP, bool PAD, bool P16, int NB>
 hipError_t attn_launch(const PagedAttnArgs& a, int items, hipStream_t st) {
   const size_t lds = (size_t)(4 * a.gs * (DP + 4) + 4 * 16 * NB * 2 + (a.held ? a.gs * a.pitch : 0)) * sizeof(float);
-  if (lds > 65536) {
+  if (lds > 49152) {
     const hipError_t e = hipFuncSetAttribute((const void*)paged_attn_kernel<DT, DP, PAD, P16, NB>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;

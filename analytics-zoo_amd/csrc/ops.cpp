@@ -3181,7 +3181,8 @@ void paged_ints(const torch::Tensor& t, const torch::Tensor& lengths, const char
 }
 
 // pools that are written must not overlap themselves or each other
-void paged_written(const torch::Tensor& kp, const torch::Tensor& vp) {
+void paged_written(const torch::Tensor& kp, const torch::Tensor& vp, const torch::Tensor& table) {
+  at::assert_no_internal_overlap(table);    // an expanded table: every row the same pages
   at::assert_no_internal_overlap(kp);
   at::assert_no_internal_overlap(vp);
   at::assert_no_partial_overlap(kp, vp);
@@ -3208,6 +3209,7 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   const bool weights = scores.has_value() && scores->defined();
   TORCH_CHECK(weights || !scores_out.has_value(), what, ": scores_out without scores");
   if (weights) {
+    at::assert_no_internal_overlap(table);    // rows that share their pages would gather into the same slots
     paged_side(*scores, kp, at::kFloat, "scores", what);
     paged_no_grad({&*scores}, what);
     if (!scores_out.has_value()) scores_out = scores;
@@ -3258,7 +3260,9 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   // Past 400 MB the caches (256 MB) hold nothing until the next token, and loads that go past them are faster: 537 MB
   // 89 us, 101 through them; 4.3 GB 636 and 713. Below, they are slower: 314 MB 84 and 81, 50 MB 14.5 and 12.2. Kv heads
   // with several blocks of query heads read everything several times: 537 MB twice 188 us, through the caches 130.
+  // Where short sequences are one work item each, their number decides by what their tables can hold.
   a.cached = hbs > 1 ? 1e30f : 4e8f / (float)(2 * c.H * c.D * c.es);
+  a.big = (float)std::min(c.B * c.cap, c.P * c.page) > a.cached;
   a.per_target = (float)(0.999 / target), a.at_once = at_once >= c.B ? at_once : 0;
   a.c = (float)(scale * 1.4426950408889634);
   check_hip(zoo_paged_attn(&a, (int)items, cur_stream()), what);
@@ -3282,7 +3286,7 @@ torch::Tensor paged_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, t
   const int64_t T = k.size(1), vec = c.D * c.es / 16;
   TORCH_CHECK(T * c.H * vec < (1LL << 31) - 256 && c.B * ((T * c.H * vec + 255) / 256 + 1) < (1LL << 24), what,
               ": too many tokens in one call");    // below 2^32 threads
-  paged_written(kp, vp);
+  paged_written(kp, vp, table);
   if (counts.has_value()) paged_ints(*counts, lengths, "counts", what);
   if (seen.has_value()) paged_ints(*seen, lengths, "seen", what);
   if (scores.has_value()) {
@@ -3321,7 +3325,7 @@ torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scor
   c10::DeviceGuard guard(kp.device());
   TORCH_CHECK(budget >= 1 && budget <= zoo::kKvMaxSlots, what, ": budget must be from 1 to 2^30");
   TORCH_CHECK(recent >= 0 && recent <= budget, what, ": recent must be from 0 to the budget");
-  paged_written(kp, vp);
+  paged_written(kp, vp, table);
   paged_ints(seen, lengths, "seen", what);
   for (const torch::Tensor* t : {&scores, &scores_out}) paged_side(*t, kp, at::kFloat, "scores", what);
   for (const torch::Tensor* t : {&positions, &positions_out}) paged_side(*t, kp, at::kInt, "positions", what);

@@ -436,6 +436,11 @@ def test_refusals(dev):
         no(paged_attention, wide, k, v, table, n)                       # 257 heads to a kv head
         no(paged_append, x, x, k, k, table, n)                          # keys and values in one place
         no(paged_append, x, x, k[:1].expand(k.shape), v, table, n)
+        one = table[:1].expand(2, -1)                                   # both rows the same pages
+        assert torch.equal(paged_attention(q, k, v, one, n)[0], paged_attention(q, k, v, table, n)[0])
+        no(paged_attention, q, k, v, one, n, scores=s)
+        no(paged_append, x, x, k, v, one, n)
+        no(paged_evict, k, v, s, p, one, n, n, 4)
         no(paged_evict, k, v, s.half(), p, table, n, n, 4)
         no(paged_evict, k, v, s, p.long(), table, n, n, 4)
 
@@ -500,3 +505,24 @@ def test_many_short_sequences(gpu):
         close(o[b:b + 1], ref, mag, 64)
         close(o2[b:b + 1], ref, mag, 64)
     assert torch.isfinite(o2[fine]).all()
+
+
+@GPU
+@pytest.mark.parametrize("longest,rows", [(40, 900), (1000, 45)])
+def test_streamed_past_the_caches(gpu, longest, rows):
+    """Batches too large for the caches take their keys and values past them, sequences that are one work item each and
+    split ones: the same results as row by row."""
+    H, D, page = 16, 128, 16
+    lengths = [longest - i % 7 for i in range(rows)]
+    assert 2 * H * D * 4 * sum(lengths) > 4e8
+    width = -(-longest // page)
+    g = torch.Generator("cuda").manual_seed(3)
+    k, v = (torch.randn(rows * width, H, page, D, generator=g, device="cuda") for _ in range(2))
+    table = torch.arange(rows * width, dtype=torch.int32, device="cuda").view(width, rows).t().contiguous()
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    q = torch.randn(rows, H, D, generator=g, device="cuda")
+    o = paged_attention(q, k, v, table, n)
+    for b in range(0, rows, rows // 5):
+        ref, mag, _ = define(q[b:b + 1], k, v, table[b:b + 1], lengths[b:b + 1])
+        close(o[b:b + 1], ref, mag, D)
+        close(paged_attention(q[b:b + 1], k, v, table[b:b + 1], n[b:b + 1]), ref, mag, D)
