@@ -33,7 +33,10 @@ def _dropout_seed(device, pdrop):
 
 def _reference(q, k, v, mask, causal, dropout_p, training):
     scale = 1.0 / math.sqrt(q.shape[-1])
-    w = torch.matmul(q, k.transpose(-1, -2)) * scale
+    kt = k.transpose(-1, -2)
+    if kt.is_cuda:      # batched 16-bit products of a transposed view have faulted on MI355X
+        kt = kt.contiguous()
+    w = torch.matmul(q, kt) * scale
     if causal:
         L, S = w.shape[-2], w.shape[-1]
         tri = torch.ones(L, S, dtype=torch.bool, device=w.device).tril(S - L)

@@ -200,6 +200,8 @@ class TransformerLayer(Layer):
         n, T = xs[0].shape
         at = list(range(cache.batch)) if rows is None else list(rows)
         counts = [T] * n if counts is None else [int(c) for c in counts]
+        if n == 0 or T == 0:
+            raise ValueError("prefill: no prompts, or none with a token")
         if len(at) != n or len(counts) != n or len(set(at)) != n:
             raise ValueError("prefill: a row of the cache and a count for each prompt")
         if not all(0 <= c <= T for c in counts):
@@ -224,7 +226,7 @@ class TransformerLayer(Layer):
         """One token of every row of ``cache``, or of the rows ``rows`` (a list of numbers): ``xs`` = [token_ids,
         position_ids] ([n]). Returns the sequence output of these tokens [n, hidden]."""
         n = cache.batch if rows is None else len(rows)
-        if xs[0].dim() != 1 or xs[0].shape[0] != n or (rows is not None and len(set(rows)) != n):
+        if n == 0 or xs[0].dim() != 1 or xs[0].shape[0] != n or (rows is not None and len(set(rows)) != n):
             raise ValueError("decode: one token for each row of the cache")
         cache.reserve(1, rows)
         sub = None if rows is None else torch.tensor(list(rows)).to(cache.k.device)

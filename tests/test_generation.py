@@ -129,6 +129,19 @@ def test_eviction_while_decoding(dev, slack):
     assert torch.allclose(total, torch.full_like(total, 20.0), atol=20 * 40 * 2.0 ** -20)
 
 
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("hidden,heads", [(64, 4), (128, 2)])
+def test_prompts_of_one_token(dev, hidden, heads):
+    t = layer(dev, hidden, heads, std=0.02)
+    tok, pos = ids(1, 3, dev)
+    with torch.no_grad():
+        want = t([tok, pos])[0]
+    cache = t.init_cache(1, max_length=3, page=1)
+    near(t.prefill([tok[:, :1], pos[:, :1]], cache)[:, 0], want[:, 0], dev, hidden, 0.02)
+    for i in (1, 2):
+        near(t.decode([tok[:, i], pos[:, i]], cache), want[:, i], dev, hidden, 0.02)
+
+
 def test_refusals():
     t = layer("cpu")
     tok, pos = ids(2, 10, "cpu")
@@ -147,6 +160,10 @@ def test_refusals():
         t.decode([tok, pos], cache)
     with pytest.raises(ValueError):
         t.decode([tok[:, 0], pos[:, 0]], cache, rows=[1, 1])
+    with pytest.raises(ValueError):
+        t.decode([tok[:0, 0], pos[:0, 0]], cache, rows=[])
+    with pytest.raises(ValueError):
+        t.prefill([tok[:, :0], pos[:, :0]], t.init_cache(2))
     with pytest.raises(ValueError):
         t.prefill([tok, pos], cache, rows=[0])
     with pytest.raises(ValueError):
