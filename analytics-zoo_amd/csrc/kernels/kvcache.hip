@@ -1065,7 +1065,8 @@ __global__ __launch_bounds__(NT) void paged_evict_select_kernel(const PagedEvict
 // Rows of more slots than one workgroup should take: the same selection with a row shared out in segments of
 // kEvictSeg, a launch for each step that needs all of the row before it. Histograms of a row add
 // up in memory (whole numbers, so in any order). 8 rows of 131k slots: 35 us in five launches, one workgroup each 590. The
-// whole eviction from 8 rows of 16384 slots takes 31 us so and 33 with a workgroup each, from 256 rows 127 and 85. STEP 0 .. 2: the digits, 3: counts of each wave's stretch, 4: the lists.
+// whole eviction from 8 rows of 16384 slots takes 31 us so and 33 with a workgroup each, from 256 rows 127 and 85.
+// STEP 0 .. 2: the digits, 3: counts of each wave's stretch, 4: the lists.
 template <int STEP>
 __global__ __launch_bounds__(256) void paged_evict_long_kernel(const PagedEvictArgs a) {
   __shared__ int hist[kEvictBins];
@@ -1184,7 +1185,8 @@ hipError_t attn_launch(const PagedAttnArgs& a, int items, hipStream_t st) {
 template <int DT, int DP, int NB>
 hipError_t attn_pick(const PagedAttnArgs& a, int items, hipStream_t st) {
   const bool p16 = a.page.d % 16 == 0;
-  if (a.D == DP) return p16 ? attn_launch<DT, DP, false, true, NB>(a, items, st) : attn_launch<DT, DP, false, false, NB>(a, items, st);
+  if (a.D == DP)
+    return p16 ? attn_launch<DT, DP, false, true, NB>(a, items, st) : attn_launch<DT, DP, false, false, NB>(a, items, st);
   return p16 ? attn_launch<DT, DP, true, true, NB>(a, items, st) : attn_launch<DT, DP, true, false, NB>(a, items, st);
 }
 
