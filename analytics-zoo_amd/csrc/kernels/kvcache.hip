@@ -376,14 +376,29 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
   uint4 kr[NS][KL];
   uint32_t vr[NS][4][VC][VW];
 
-  auto page_of = [&](int slot) {
+  [[maybe_unused]] auto page_of = [&](int slot) {
     const int p = fixed(table)[fdiv(slot, a.page)];
     const bool ok = (unsigned)p < (unsigned)a.pages;
     bad |= !ok;
     return ok ? p : 0;
   };
+  // Pages of any size: lane l looks up slot l of the tile, the page number one tile ahead, and the rows' offsets go from
+  // lane to lane (54 rows of up to 29k slots, 24 heads of 64, pages of 100: 55 us; with look-ups by every lane for itself,
+  // five a subtile, 100; pages of 64 53).
+  int ahead_id = 0;
+  long k_at = 0, v_at = 0;
+  auto slot_of = [&](int base) { return min(base + (lane & (T::TS - 1)), w.s1 - 1); };
   auto load_k = [&](int base, auto nt) {
     constexpr bool NT = decltype(nt)::value;
+    if constexpr (!P16) {
+      const int s = slot_of(base);
+      const bool ok = (unsigned)ahead_id < (unsigned)a.pages;
+      bad |= !ok;
+      const long id = ok ? ahead_id : 0, off = s - fdiv(s, a.page) * a.page.d;
+      k_at = (id * a.ks.page + off * a.ks.row) * ES;
+      v_at = (id * a.vs.page + off * a.vs.row) * ES;
+      ahead_id = table[fdiv(slot_of(base + T::GRAIN), a.page)];
+    }
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
       const char* p;
@@ -391,8 +406,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
         const int s = min(base + 16 * u, (w.s1 - 1) & ~15);
         p = kb + ((long)uni(page_of(s)) * a.ks.page + (long)(s - fdiv(s, a.page) * a.page.d) * a.ks.row) * ES + klane;
       } else {
-        const int s = min(base + 16 * u + row, w.s1 - 1);
-        p = kb + ((long)page_of(s) * a.ks.page + (long)(s - fdiv(s, a.page) * a.page.d) * a.ks.row) * ES + quad * 16;
+        p = kb + __shfl(k_at, 16 * u + row, 64) + quad * 16;
       }
 #pragma unroll
       for (int i = 0; i < KL; ++i) {
@@ -421,8 +435,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
         if constexpr (P16) {
           p += (long)r * a.vs.row * ES;
         } else {
-          const int s = min(base + 16 * u + 4 * quad + r, w.s1 - 1);
-          p += ((long)page_of(s) * a.vs.page + (long)(s - fdiv(s, a.page) * a.page.d) * a.vs.row) * ES;
+          p += __shfl(v_at, 16 * u + 4 * quad + r, 64);
         }
 #pragma unroll
         for (int c = 0; c < VC; ++c) {
@@ -454,6 +467,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
   auto stream = [&](auto nt) {
     int base = w.s0 + wave * T::TS;
     if (base < w.s1) {
+      if constexpr (!P16) ahead_id = table[fdiv(slot_of(base), a.page)];
       load_k(base, nt);
       load_v(base, nt);
     }
