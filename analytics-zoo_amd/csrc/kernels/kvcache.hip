@@ -595,8 +595,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
       if (more) load_v(base + T::GRAIN, nt);
     }
   };
-  if (P16 && !PAD && w.big)
-    stream(std::bool_constant<P16 && !PAD>{});
+  if (!PAD && w.big)
+    stream(std::bool_constant<!PAD>{});
   else
     stream(std::false_type{});
   const bool weights = a.held || (w.n == 1 && a.logits != nullptr && a.G <= W);
