@@ -92,6 +92,10 @@ def paged_evict(k_pages, v_pages, scores, positions, page_table, lengths, seen, 
                       positions_out)
 
 
+def _capturing(t):
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class PagedKVCache:
     """The caches of all layers of a model that generates for up to ``batch`` sequences at a time, and the host's book
     of their pages. The layers share one page table: layer ``i`` owns the kv heads ``i * kv_heads ..`` of the pools, so
@@ -153,6 +157,8 @@ class PagedKVCache:
             raise RuntimeError("PagedKVCache: a sequence would be longer than max_length = %d slots" % self.max_length)
         if sum(max(0, w - len(self._pages[r])) for r, w in zip(rows, want)) > len(self._free):
             raise RuntimeError("PagedKVCache: no pages left")
+        if _capturing(self.k) and any(w > len(self._pages[r]) for r, w in zip(rows, want)):
+            raise RuntimeError("PagedKVCache: a captured step cannot take pages: reserve() them before the capture")
         for r, w in zip(rows, want):
             n = len(self._pages[r])
             if w > n:
@@ -211,7 +217,7 @@ class PagedKVCache:
                           self.budget, self.recent)
         self.lengths.copy_(new)
         self._slots = [min(n, self.budget) for n in self._slots]
-        if self.k.is_cuda and torch.cuda.is_current_stream_capturing():
+        if _capturing(self.k):
             return
         keep = -(-(self.budget + self.slack + 1) // self.page)
         for r, own in enumerate(self._pages):

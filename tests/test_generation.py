@@ -261,6 +261,17 @@ def test_a_step_by_hand(gpu):
     assert torch.equal(out["cpu"][1], out["cuda"][1]) and out["cpu"][2].tolist() == [20, 20] == out["cuda"][2].tolist()
 
 
+def test_a_capture_takes_no_pages(monkeypatch):
+    import zoo.ops.kvcache as kvcache
+    c = PagedKVCache(1, 2, 20, 1, 8, page=4, device="cpu")
+    c.reserve(4)
+    monkeypatch.setattr(kvcache, "_capturing", lambda t: True)
+    c.reserve(4)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        c.reserve(5)
+    assert [len(own) for own in c._pages] == [1, 1]
+
+
 def test_the_book_on_its_own():
     c = PagedKVCache(1, 2, 20, 1, 8, page=4, device="cpu")
     c.reserve([20, 3])
