@@ -21,8 +21,11 @@
 //               16-slot halves for one dim; it loads 8 dims of each of these 8 slots (16 bytes a row, 16
 //               lanes to a row, 256 bytes contiguous) and transposes the 8 x 8 block in its registers
 //               with v_perm: MFMA e takes dim 8 (l % 16) + e.
-// P is fed as the sum of two 16-bit numbers: rounding it to one would cost an error as large as the
-// output's own rounding.
+// P is fed as the sum of three bfloat16 numbers, which hold all 24 bits of it, or of two float16 numbers (22 bits):
+// rounding it to one would cost an error as large as the output's own rounding, and two bfloat16 numbers (16 bits) still
+// turn one in 200 of the outputs' roundings. The third costs nothing where HBM is the bound (64 sequences of 16k slots 633 us
+// with two and three), and some where latency is (32 of up to 512 with weights 12.6 us and 13.1, 200 of 500 with pages of 7
+// 50 and 55).
 //
 // The slots of all sequences are cut into equal chunks, one per workgroup, whose number aims at
 // filling the chip whatever the batch and the lengths (find_work): lengths are only known on the
@@ -45,6 +48,7 @@ namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // NT: past the caches, for what will not be read again before it would have left them anyway
@@ -224,21 +228,39 @@ ZOO_DEV f32x4 mma16(const uint4& x, const uint4& y, const f32x4& c) {
                                                   0);
 }
 
-// Two weights as packed 16-bit numbers, rounded towards zero, and what that left over, packed too. The rest is
-// kept above zero (by less than 2^-35 of the largest weight), so that an infinite value times a weight stays
-// infinite: a rest of 0, or a negative one, would make it NaN.
+// Weights are held times this. Sums of up to 2^30 weighted values stay finite even for the type's largest values
+// (bfloat16 and float32: 2^-32), and float16 parts hold weights down to 2^-38 of the wave's largest (2^15, below its 65504).
 template <int DT>
-ZOO_DEV void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+constexpr float kWeight = DT == kF16 ? 0x1p15f : 0x1p-32f;
+template <int DT>
+constexpr float kWeightLog = DT == kF16 ? 15.f : -32.f;
+
+ZOO_DEV uint32_t high16(float x, float y) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); }
+// the upper 16 bits of the float next to x on the side of zero; of 0 for 0
+ZOO_DEV float below16(float x) { return __uint_as_float(__builtin_elementwise_sub_sat(__float_as_uint(x), 1u) & 0xffff0000u); }
+
+// Two weights as packed 16-bit numbers whose sum they are. Each part is cut off so that something is left for the
+// next one: an infinite value times a weight is then infinite in every part, where a part of 0 would make it NaN.
+// Only a weight of 0 has parts of 0.
+// bfloat16: 8 bits in each of three parts, nothing is lost. float16: 11 bits in each of two, an error of 2^-22 of the weight
+// and 2^-25 (2^-40 of the wave's largest weight, in either direction, with no sign to add up in); what is below 2^-23
+// goes into the second part alone.
+template <int DT>
+constexpr int kParts = DT == kBf16 ? 3 : 2;
+
+template <int DT>
+ZOO_DEV void split(float x, float y, uint32_t (&part)[kParts<DT>]) {
   if constexpr (DT == kBf16) {
-    const uint32_t xi = __float_as_uint(x), yi = __float_as_uint(y);
-    hi = __builtin_amdgcn_perm(yi, xi, 0x07060302u);
-    lo = pack2bf(fmaxf(x - __uint_as_float(xi & 0xffff0000u), 0x1p-126f),
-                 fmaxf(y - __uint_as_float(yi & 0xffff0000u), 0x1p-126f));
+    const float x0 = below16(x), y0 = below16(y), xr = x - x0, yr = y - y0;
+    const float x1 = below16(xr), y1 = below16(yr);
+    part[0] = high16(x0, y0);
+    part[1] = high16(x1, y1);
+    part[2] = high16(xr - x1, yr - y1);
   } else {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
-    const auto r = __builtin_amdgcn_cvt_pkrtz(fmaxf(x - (float)h[0], 0x1p-24f), fmaxf(y - (float)h[1], 0x1p-24f));
-    hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, r);
+    constexpr float kLess = 1.f - 0x1p-22f;
+    const auto h = __builtin_amdgcn_cvt_pkrtz(fmaxf(fmaf(x, kLess, -0x1p-24f), 0.f), fmaxf(fmaf(y, kLess, -0x1p-24f), 0.f));
+    part[0] = __builtin_bit_cast(uint32_t, h);
+    part[1] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)(x - (float)h[0]), (_Float16)(y - (float)h[1])});
   }
 }
 
@@ -317,9 +339,10 @@ ZOO_DEV void gather_weights(const PagedAttnArgs& a, int b, int hk, int s0, int s
 
 // DP: the head width rounded up; PAD: it was rounded; P16: pages of a multiple of 16 rows, so that a
 // 16-slot subtile lies in one page and its address is wave-uniform. Other page sizes look up a page per
-// slot. NB: blocks of 16 query heads that share what was loaded.
+// slot. NB: blocks of 16 query heads that share what was loaded. Three workgroups to a CU where the registers allow it; in 16
+// bits with pages of any size they do not without spilling (200 sequences of 500 slots, pages of 7: two 55 us, three 60).
 template <int DT, int DP, bool PAD, bool P16, int NB>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP == 128 && PAD) ? 2 : 3) void paged_attn_kernel(
+__global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT != kF32 && !P16) || (DT == kF32 && DP == 128 && PAD) ? 2 : 3) void paged_attn_kernel(
     const PagedAttnArgs a) {
   using T = Tile<DT, DP>;
   constexpr int NS = T::NS, KL = T::KL, VC = T::VC, VW = T::VW, VE = T::VE, NA = T::NA, ES = T::ES;
@@ -349,8 +372,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
     for (int i = threadIdx.x; i < gb * D; i += 256) store_out<DT>(a.o, out0 + i, x);
     return;
   }
-  // fp16 cannot hold small weights: they are kept times 2^12 (their maximum is 1, and 16 * 2^12 < 2^16)
-  constexpr float kUp = DT == kF16 ? 12.f : 0.f;
 
   // Q^T: heads row, 16 + row, the dims that K's loads bring. Heads and dims that are not there are zero.
   uint4 q[NB][KL];
@@ -533,7 +554,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
         for (int u = 0; u < NS; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            s[n][u][r] = pow2(s[n][u][r] - mu + kUp);
+            s[n][u][r] = pow2(s[n][u][r] - mu) * kWeight<DT>;
             l[n] += s[n][u][r];
           }
       }
@@ -566,14 +587,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
       } else {
 #pragma unroll
         for (int u = 0; u < NS; u += 2) {
-          uint4 hi[NB], lo[NB];
+          uint32_t w2[NB][4][kParts<DT>];
 #pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            split2<DT>(s[n][u][0], s[n][u][1], hi[n].x, lo[n].x);
-            split2<DT>(s[n][u][2], s[n][u][3], hi[n].y, lo[n].y);
-            split2<DT>(s[n][u + 1][0], s[n][u + 1][1], hi[n].z, lo[n].z);
-            split2<DT>(s[n][u + 1][2], s[n][u + 1][3], hi[n].w, lo[n].w);
-          }
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) split<DT>(s[n][u + i / 2][2 * (i & 1)], s[n][u + i / 2][2 * (i & 1) + 1], w2[n][i]);
 #pragma unroll
           for (int c = 0; c < VC; ++c)
 #pragma unroll
@@ -585,10 +603,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
               x.z = __builtin_amdgcn_perm(vr[u + 1][1][c][e / 2], vr[u + 1][0][c][e / 2], sel);
               x.w = __builtin_amdgcn_perm(vr[u + 1][3][c][e / 2], vr[u + 1][2][c][e / 2], sel);
 #pragma unroll
-              for (int n = 0; n < NB; ++n) {
-                acc[n][c * VE + e] = mma16<DT>(x, hi[n], acc[n][c * VE + e]);
-                acc[n][c * VE + e] = mma16<DT>(x, lo[n], acc[n][c * VE + e]);
-              }
+              for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int p = 0; p < kParts<DT>; ++p)
+                  acc[n][c * VE + e] =
+                      mma16<DT>(x, make_uint4(w2[n][0][p], w2[n][1][p], w2[n][2][p], w2[n][3][p]), acc[n][c * VE + e]);
             }
         }
       }
@@ -649,7 +668,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT == kF32 && DP =
         a.part_ml[((long)item_of(a) * W + g) * 2] = top;
         a.part_ml[((long)item_of(a) * W + g) * 2 + 1] = sum;
       }
-      lse[g] = top + log2f(sum) - kUp;
+      lse[g] = top + log2f(sum) - kWeightLog<DT>;
     }
   }
   if (weights) {
@@ -698,7 +717,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Pag
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) merge(m, l, x, __shfl_xor(m, o, 64), __shfl_xor(l, o, 64), 0.f);
-      if (g < a.G && (tid & 15) == 0) lse[g] = m + log2f(l) - (a.dtype == kF16 ? 12.f : 0.f);
+      if (g < a.G && (tid & 15) == 0) lse[g] = m + log2f(l) - (a.dtype == kF16 ? kWeightLog<kF16> : kWeightLog<kF32>);
     }
     if (w.n == 1) __syncthreads();
   }

@@ -526,3 +526,60 @@ def test_streamed_past_the_caches(gpu, longest, rows):
         ref, mag, _ = define(q[b:b + 1], k, v, table[b:b + 1], lengths[b:b + 1])
         close(o[b:b + 1], ref, mag, D)
         close(paged_attention(q[b:b + 1], k, v, table[b:b + 1], n[b:b + 1]), ref, mag, D)
+
+
+# ---------------------------------------------------------------------------- weights in full
+def _cancelling(dev, dtype, lengths_of_two=64, D=64):
+    """Two slots whose weighted values cancel but for the rounding of the second value, so that an output is small against
+    what it is summed from and shows how exactly the weights were kept. One product makes a logit: it is exact."""
+    g = torch.Generator().manual_seed(11)
+    B, H = lengths_of_two, 4
+    q, k, v, table, n = make(B, H, 1, D, 16, [2] * B, FL, "cpu", seed=1)
+    q.zero_()
+    q[:, :, 0] = 1.0
+    a = (torch.rand(B, H, 2, generator=g) * 2 - 1).to(dtype).float()
+    v0 = (torch.randn(B, H, D, generator=g)).to(dtype).float()
+    w = torch.softmax(a.double(), -1)
+    v1 = (-v0.double() * w[..., :1] / w[..., 1:]).to(dtype).float()
+    for b in range(B):
+        p = int(table[b, 0])
+        k[p, :, :2] = 0.0
+        k[p, :, :2, 0] = a[b]
+        v[p, :, 0], v[p, :, 1] = v0[b], v1[b]
+    return [t.to(dtype).to(dev) for t in (q, k, v)] + [table.to(dev), n.to(dev)]
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("dtype", [BF, HF, FL])
+def test_weights_are_kept_to_float32(dev, dtype):
+    """A logit of at most 1 is multiplied by log2(e) and taken off the maximum, 2^-24 relative each, which moves a weight
+    by at most 2^-22; its exponential and its place in the sums add 2^-23 each, a split into 16-bit parts at most 2^-22. So
+    an output is off by half a step and at most 2^-20 of what it is summed from. (Weights of 16 bits are off by up to
+    2^-16, and the values' own rounding leaves outputs of 2^-9 of their parts in bfloat16, whose half step is
+    2^-17.)"""
+    args = _cancelling(dev, dtype)
+    ref, mag, _ = define(*[t.cpu() for t in args[:4]], [2] * 64, scale=1.0)
+    o = paged_attention(*args, scale=1.0).double().cpu()
+    tol = torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -20 * mag + (2.0 ** -25 if dtype == HF else 0.0)
+    assert ((o - ref).abs() <= tol).all(), ((o - ref).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("dtype,logit", [(BF, -500.0), (HF, -500.0), (FL, -500.0), (BF, -100.0), (HF, -60.0)])
+def test_slots_without_weight_add_nothing(dev, dtype, logit):
+    """One slot has all the weight and a small value, a thousand others hold the type's largest values and a weight that is 0
+    in float32 (exp -500), or too small to count: 1000 e^-100 3e38 is below 1e-2 of 2^-4's half step in
+    bfloat16, 1000 e^-60 65504 below 1e-14 of it in float16."""
+    n = 1001
+    q, k, v, table, lens = make(1, 2, 3, 64, 16, [n], FL, "cpu", seed=2)
+    big = torch.finfo(dtype).max if dtype != BF or logit == -500.0 else 2.0 ** 100
+    q.zero_()
+    q[:, :, 0] = 1.0
+    k.zero_()
+    k[..., 0] = logit
+    v.fill_(big)
+    k[int(table[0, 0]), :, 0, 0] = 0.0
+    v[int(table[0, 0]), :, 0] = 2.0 ** -4
+    q, k, v = (t.to(dtype).to(dev) for t in (q, k, v))
+    o = paged_attention(q, k, v, table.to(dev), lens.to(dev), scale=1.0).double().cpu()
+    assert ((o - 2.0 ** -4).abs() <= torch.finfo(dtype).eps / 2 * 2.0 ** -4).all(), (o - 2.0 ** -4).abs().max().item()
