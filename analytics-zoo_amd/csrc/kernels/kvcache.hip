@@ -311,9 +311,15 @@ ZOO_DEV Ahead weights_ahead(const PagedAttnArgs& a, int b, int hk, int s, int s1
   return x;
 }
 
+// The log of the sums that stands for a sequence with a bad page: its slots gather nothing, on good pages either. What
+// data can give is finite, -inf or NaN. (Where it is summed from, a maximum of NaN stands for one: a maximum that fmaxf
+// found is never NaN.)
+constexpr float kBadLse = INFINITY;
+
 // `logit`: of the kv head's first query head, in memory or in LDS
 ZOO_DEV void gather_weights(const PagedAttnArgs& a, int b, int hk, int s0, int s1, Ahead x, const float* lse,
                             const float* logit) {
+  if (lse[0] == kBadLse) return;    // pages are a sequence's: all its heads say so
   const int G = a.G, step = blockDim.x;
   float* out = a.scores_out + (long)hk * a.sos.head;
   for (int s = s0 + threadIdx.x; s < s1; s += kWays * step) {
@@ -629,7 +635,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT != kF32 && !P16
   for (int n = 0; n < NB; ++n) {
     l[n] += __shfl_xor(l[n], 16, 64);
     l[n] += __shfl_xor(l[n], 32, 64);
-    if (wrong) l[n] = __builtin_nanf("");
     const int h = 16 * n + row;
     if (h < gb) {
 #pragma unroll
@@ -638,7 +643,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT != kF32 && !P16
         for (int r = 0; r < 4; ++r)
           lds[(wave * gb + h) * LD + (i / VE) * (16 * VE) + (quad * 4 + r) * VE + i % VE] = acc[n][i][r];
       if (quad == 0) {
-        ml[(wave * W + h) * 2] = m[n];
+        ml[(wave * W + h) * 2] = wrong ? __builtin_nanf("") : m[n];   // and so everything that is summed with it
         ml[(wave * W + h) * 2 + 1] = l[n];
       }
     }
@@ -647,8 +652,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT != kF32 && !P16
   for (int i = threadIdx.x; i < gb * DP; i += 256) {
     const int g = i / DP, d = i & (DP - 1);
     float top = -INFINITY;
+    bool bad_page = false;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) top = fmaxf(top, ml[(x * W + g) * 2]);
+    for (int x = 0; x < 4; ++x) {
+      top = fmaxf(top, ml[(x * W + g) * 2]);
+      bad_page |= isnan(ml[(x * W + g) * 2]);
+    }
     const float mu = top == -INFINITY ? 0.f : top;
     float sum = 0.f, o = 0.f;
 #pragma unroll
@@ -665,10 +674,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT != kF32 && !P16
     }
     if (d == 0) {
       if (a.part_ml != nullptr) {
-        a.part_ml[((long)item_of(a) * W + g) * 2] = top;
+        a.part_ml[((long)item_of(a) * W + g) * 2] = bad_page ? __builtin_nanf("") : top;
         a.part_ml[((long)item_of(a) * W + g) * 2 + 1] = sum;
       }
-      lse[g] = top + log2f(sum) - kWeightLog<DT>;
+      lse[g] = bad_page ? kBadLse : top + log2f(sum) - kWeightLog<DT>;
     }
   }
   if (weights) {
@@ -711,13 +720,19 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Pag
       const int g = g0 + (tid >> 4);
       const float* ml = a.part_ml + ((long)(w.first + g / a.wide) * a.wide + g % a.wide) * 2;
       float m = -INFINITY, l = 0.f, x = 0.f;
+      bool bad_page = false;
       if (g < a.G) {
 #pragma unroll 4
-        for (int i = tid & 15; i < w.n; i += 16) merge(m, l, x, ml[i * next], ml[i * next + 1], 0.f);
+        for (int i = tid & 15; i < w.n; i += 16) {
+          const float top = ml[i * next];
+          bad_page |= isnan(top);
+          merge(m, l, x, top, ml[i * next + 1], 0.f);
+        }
       }
+      bad_page = __ballot(bad_page) >> (tid & 48) & 0xffff;   // of the 16 threads of this head
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) merge(m, l, x, __shfl_xor(m, o, 64), __shfl_xor(l, o, 64), 0.f);
-      if (g < a.G && (tid & 15) == 0) lse[g] = m + log2f(l) - (a.dtype == kF16 ? kWeightLog<kF16> : kWeightLog<kF32>);
+      if (g < a.G && (tid & 15) == 0) lse[g] = bad_page ? kBadLse : m + log2f(l) - (a.dtype == kF16 ? kWeightLog<kF16> : kWeightLog<kF32>);
     }
     if (w.n == 1) __syncthreads();
   }

@@ -16,8 +16,8 @@ eviction each kv head may hold other tokens.
 
 Lengths and tables are read on the device only, so a decoding step can be captured into a hipGraph. What
 cannot be checked on the host is never followed: a length below 0 or past the table (or ``max_length``), or
-a page id outside the pools, makes the attention of that sequence NaN; its tokens on such pages are not
-written, and it is not evicted from. A page that is written (by ``paged_append``, ``paged_evict`` or as
+a page id outside the pools, makes the attention of that sequence NaN, and its slots gather no weight; its
+tokens on such pages are not written, and it is not evicted from. A page that is written (by ``paged_append``, ``paged_evict`` or as
 ``scores_out``) must belong to one row of the table only, and once; pages that are only read may be
 shared.
 

@@ -583,3 +583,47 @@ def test_slots_without_weight_add_nothing(dev, dtype, logit):
     q, k, v = (t.to(dtype).to(dev) for t in (q, k, v))
     o = paged_attention(q, k, v, table.to(dev), lens.to(dev), scale=1.0).double().cpu()
     assert ((o - 2.0 ** -4).abs() <= torch.finfo(dtype).eps / 2 * 2.0 ** -4).all(), (o - 2.0 ** -4).abs().max().item()
+
+
+# ---------------------------------------------------------------------------- weights of a sequence with a bad page
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("H,G,D,page,dtype,lengths,width", [
+    (2, 2, 64, 16, BF, [40, 33, 20, 70], None),          # one work item each, products in LDS
+    (1, 16, 64, 16, BF, [300, 290, 20, 310], None),      # products in memory
+    (2, 2, 128, 16, HF, [900, 830, 20, 1200], 400),      # split
+    (1, 40, 64, 16, BF, [40, 33, 20, 70], None),         # several blocks of query heads
+    (1, 70, 128, 16, BF, [900, 830, 0, 1200], 300),      # ... and split
+    (3, 1, 80, 7, FL, [700, 650, 9, 800], 500),
+])
+def test_bad_pages_leave_the_gathered_weights(dev, H, G, D, page, dtype, lengths, width):
+    """A sequence that names a bad page gathers nothing, on its good pages neither; the others do as ever. NaN that the
+    data holds comes through."""
+    q, k, v, table, n = make(4, H, G, D, page, lengths, dtype, dev, width=width)
+    start = torch.rand(k.shape[:3]).to(dev)
+    good = torch.full_like(start, -3.0)
+    o = paged_attention(q, k, v, table, n, scores=start, scores_out=good)
+    rows = [[(int(table[b, s // page]), s % page) for s in range(m)] for b, m in enumerate(lengths)]
+    for at, bad in ((0, -1), (1, k.shape[0]), (lengths[1] // page, -5)):
+        t2 = table.clone()
+        t2[1, at] = bad
+        want, kept = good.clone(), start.clone()
+        for p, r in rows[1]:
+            want[p, :, r] = -3.0
+        for b in (0, 2, 3):
+            for p, r in rows[b]:
+                kept[p, :, r] = good[p, :, r]
+        out = torch.full_like(start, -3.0)
+        o2 = paged_attention(q, k, v, t2, n, scores=start, scores_out=out)
+        assert torch.isnan(o2[1]).all() and torch.equal(o2[[0, 2, 3]], o[[0, 2, 3]])
+        assert torch.equal(out, want), at
+        here = start.clone()
+        paged_attention(q, k, v, t2, n, scores=here)
+        assert torch.equal(here, kept), at
+    p, r = rows[3][5]
+    k[p, 0, r, 3] = float("nan")
+    out = torch.full_like(start, -3.0)
+    o2 = paged_attention(q, k, v, table, n, scores=start, scores_out=out)
+    assert torch.isnan(o2[3, :G]).all() and torch.equal(o2[:3], o[:3])
+    assert all(bool(torch.isnan(out[p, 0, r])) for p, r in rows[3])
+    assert all(torch.equal(out[p, :, r], good[p, :, r]) for b in range(3) for p, r in rows[b])
+    assert all(torch.equal(out[p, 1:, r], good[p, 1:, r]) for p, r in rows[3])
