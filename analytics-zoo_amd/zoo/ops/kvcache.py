@@ -105,9 +105,12 @@ class PagedKVCache:
     number, by default ``batch`` sequences of ``max_length`` slots. With ``budget``, sequences longer than ``budget +
     slack`` slots are cut down to ``budget`` after a step; their last ``recent`` tokens stay.
 
-    A step of every layer: :meth:`append`, :meth:`attend` per layer, then :meth:`advance`. Inside a captured hipGraph
-    no page can be taken, so ``reserve`` what the replays will need first, and tell the host's book about them
-    with :meth:`replayed`."""
+    A step of every layer: :meth:`append`, :meth:`attend` per layer, then :meth:`advance`.
+
+    Inside a captured hipGraph no page can be taken. So ``reserve`` what a step needs before the capture and before each
+    replay (which raises where a replay could not be carried out), and tell the host's book about the replay with
+    :meth:`replayed` after it. Between replays rows may be released and filled again. A captured step is laid out for rows
+    of ``max_length`` slots, or of all ``pages``: that bounds its workspace, so make it no larger than needed."""
 
     def __init__(self, n_layer, batch, max_length, kv_heads, head_dim, page=64, pages=None, budget=None, recent=None,
                  slack=0, dtype=None, device=None):
@@ -175,8 +178,12 @@ class PagedKVCache:
             self.seen[r] = 0
 
     def _table(self):
-        # no wider than the pages in hand, which bounds the operators' workspace
-        return self.page_table[:, :max(1, max(len(own) for own in self._pages))]
+        # No wider than the pages in hand, which bounds the operators' workspace. A captured step keeps the width it was
+        # captured with, so it gets all that a row can come to own.
+        width = max(len(own) for own in self._pages)
+        if _capturing(self.k):
+            width = min(self.page_table.shape[1], self.k.shape[0])
+        return self.page_table[:, :max(1, width)]
 
     def append(self, i, k, v, counts=None, rows=None):
         """``paged_append`` to layer ``i`` of all rows, or of the ``rows`` (int64 [n] on the device); returns the new

@@ -325,3 +325,58 @@ def test_captured_operators_over_long_rows(gpu):
         for a, b in zip(pools, eager):
             assert torch.equal(a.nan_to_num() if a.is_floating_point() else a, b.nan_to_num() if b.is_floating_point() else b)
     assert torch.isfinite(junk)
+
+
+def test_a_captured_step_sees_the_whole_table(monkeypatch):
+    import zoo.ops.kvcache as kvcache
+    c = PagedKVCache(1, 2, 40, 1, 8, page=4, device="cpu")
+    few = PagedKVCache(1, 2, 40, 1, 8, page=4, pages=3, device="cpu")
+    for x in (c, few):
+        x.reserve(4)
+        assert x._table().shape == (2, 1)
+    monkeypatch.setattr(kvcache, "_capturing", lambda t: True)
+    assert c._table().shape == (2, 10) and few._table().shape == (2, 3)      # no row can ever have more
+    assert c._table().data_ptr() == c.page_table.data_ptr()
+
+
+@pytest.mark.gpu
+def test_captured_step_of_rows_that_come_and_go(gpu):
+    """After the capture a row leaves and a prompt longer than any before takes its place, and rows take pages as they
+    grow: the replays go on as eager steps do."""
+    t = layer("cuda", blocks=2)
+    tok, pos = ids(3, 60, "cuda")
+    caches = [t.init_cache(3, max_length=70, page=4) for _ in range(2)]
+    for c in caches:
+        t.prefill([tok[:, :6], pos[:, :6]], c)
+    eager, static = caches
+    x, p = tok[:, 6].clone(), pos[:, 6].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    spare = t.init_cache(3, max_length=70, page=4)
+    with torch.cuda.stream(side):
+        t.decode([x, p], spare)
+    torch.cuda.current_stream().wait_stream(side)
+    static.reserve(1)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = t.decode([x, p], static)
+    g.replay()
+    assert torch.equal(y, t.decode([x, p], eager))
+    at = [7, 7, 7]
+    for i in range(30):
+        if i == 3:
+            for c in caches:
+                c.release([1])
+                t.prefill([tok[1:2, :31], pos[1:2, :31]], c, rows=[1])
+            at[1] = 31
+        x.copy_(torch.stack([tok[b, at[b]] for b in range(3)]))
+        p.copy_(torch.stack([pos[b, at[b]] for b in range(3)]))
+        static.reserve(1)
+        g.replay()
+        static.replayed(1)
+        junk = torch.randn(512, 512, device="cuda") @ torch.randn(512, 512, device="cuda")
+        want = t.decode([x, p], eager)
+        at = [n + 1 for n in at]
+        assert torch.equal(y, want), i
+        assert static.lengths.tolist() == eager.lengths.tolist() == at == static._slots
+    assert torch.isfinite(junk).all()
