@@ -236,10 +236,10 @@ class PagedKVCache:
     def replayed(self, tokens=1, evicts=False):
         """Tells the host's book that a captured step, which gave every row ``tokens`` tokens and ended with an eviction
         if ``evicts``, was replayed; the capture itself has been counted, as the first replay."""
-        slots = [min(n + tokens, self.budget) if evicts else n + tokens for n in self._slots]
+        slots = [n + tokens for n in self._slots]      # in use before the eviction
         if any(n > len(own) * self.page for n, own in zip(slots, self._pages)):
             raise RuntimeError("PagedKVCache: the replayed step ran past the pages that were reserved for it")
-        self._slots = slots
+        self._slots = [min(n, self.budget) for n in slots] if evicts else slots
 
 
 # ---------------------------------------------------------------------------- PyTorch implementation

@@ -380,3 +380,15 @@ def test_captured_step_of_rows_that_come_and_go(gpu):
         assert torch.equal(y, want), i
         assert static.lengths.tolist() == eager.lengths.tolist() == at == static._slots
     assert torch.isfinite(junk).all()
+
+
+def test_the_book_of_replays_counts_the_token_before_its_eviction():
+    c = PagedKVCache(1, 1, 20, 1, 8, page=4, budget=4, device="cpu")
+    c.reserve(4)
+    c._slots = [4]
+    with pytest.raises(RuntimeError, match="reserved"):
+        c.replayed(1, evicts=True)          # its token had no page
+    assert c._slots == [4]
+    c.reserve(1)
+    c.replayed(1, evicts=True)
+    assert c._slots == [4] and len(c._pages[0]) == 2
