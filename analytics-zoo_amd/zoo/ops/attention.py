@@ -15,6 +15,7 @@ import math
 import torch
 
 from zoo.ops._native import available, native
+from zoo.ops.bmm import matmul
 from zoo.ops.pointwise import _seed
 
 
@@ -33,10 +34,7 @@ def _dropout_seed(device, pdrop):
 
 def _reference(q, k, v, mask, causal, dropout_p, training):
     scale = 1.0 / math.sqrt(q.shape[-1])
-    kt = k.transpose(-1, -2)
-    if kt.is_cuda:      # batched 16-bit products of a transposed view have faulted on MI355X
-        kt = kt.contiguous()
-    w = torch.matmul(q, kt) * scale
+    w = matmul(q, k.transpose(-1, -2)) * scale
     if causal:
         L, S = w.shape[-2], w.shape[-1]
         tri = torch.ones(L, S, dtype=torch.bool, device=w.device).tril(S - L)
@@ -46,7 +44,7 @@ def _reference(q, k, v, mask, causal, dropout_p, training):
     p = torch.softmax(w.float(), dim=-1).to(q.dtype)
     if dropout_p > 0 and training:
         p = torch.nn.functional.dropout(p, dropout_p)
-    return torch.matmul(p, v)
+    return matmul(p, v)
 
 
 class _FlashAttnFn(torch.autograd.Function):

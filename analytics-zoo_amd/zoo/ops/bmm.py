@@ -45,4 +45,42 @@ def bmm(a, b):
     return torch.matmul(a, b)
 
 
-__all__ = ["bmm"]
+def _right_in_rows(t):
+    """Whether a right operand is to have contiguous rows: the library's batched products in bfloat16 have faulted the GPU
+    when it was a transposed view. float16 shares their code path, 32 bits do not."""
+    return t.is_cuda and t.dtype in (torch.bfloat16, torch.float16)
+
+
+def _rows(t):
+    if t.stride(-1) == 1 and t.stride(-2) >= t.size(-1):
+        return t
+    return t.contiguous().view(-1).view(t.shape)    # a dimension of 1 keeps any stride, but not through a flat view
+
+
+class _MatmulFn(torch.autograd.Function):
+    """Both products of the backward have a transposed operand: they go the same way (so does their own backward)."""
+
+    @staticmethod
+    def forward(ctx, a, b):
+        ctx.save_for_backward(a, b)
+        return torch.matmul(a, _rows(b))
+
+    @staticmethod
+    def backward(ctx, dc):
+        a, b = ctx.saved_tensors
+        da = matmul(dc, b.transpose(-1, -2)).sum_to_size(a.shape) if ctx.needs_input_grad[0] else None
+        db = matmul(a.transpose(-1, -2), dc).sum_to_size(b.shape) if ctx.needs_input_grad[1] else None
+        return da, db
+
+
+def matmul(a, b):
+    """``torch.matmul`` in the operands' own type. Batched products of 16 bits on the GPU get a right operand with
+    contiguous rows, in the backward too; everything else is left to torch."""
+    if a.dim() < 2 or b.dim() < 2 or (a.dim() == 2 and b.dim() == 2) or not _right_in_rows(b):
+        return torch.matmul(a, b)
+    if b.dim() == 2:        # one plain product of all rows
+        return torch.matmul(a.reshape(-1, a.shape[-1]), b).reshape(*a.shape[:-1], b.shape[-1])
+    return _MatmulFn.apply(a, b)
+
+
+__all__ = ["bmm", "matmul"]

@@ -22,6 +22,7 @@ import torch.nn.functional as F
 
 from zoo import ops
 from zoo.ops import layers as ops_layers
+from zoo.ops.bmm import matmul
 from zoo.pipeline.api.keras.base import Layer, apply_activation, check_activation, init_tensor, to_shape
 
 
@@ -384,6 +385,11 @@ class Convolution3D(Layer):
 Conv3D = Convolution3D
 
 
+def _per_position(x, w):
+    """[L, N, K] times each position's own weight [L, K, O], as [N, L, O]."""
+    return matmul(x, w).transpose(0, 1)
+
+
 class LocallyConnected2D(Layer):
     """Unshared-weight 2-D conv via unfold + batched GEMM."""
 
@@ -410,7 +416,7 @@ class LocallyConnected2D(Layer):
     def call(self, x):
         xc = x if self.dim_ordering == "th" else x.permute(0, 3, 1, 2)
         cols = F.unfold(xc, self.kernel, stride=self.subsample)          # [N, Kd, L]
-        y = torch.einsum("nkl,lko->nlo", cols, self.weight.to(cols.dtype))
+        y = _per_position(cols.permute(2, 0, 1), self.weight.to(cols.dtype))
         if self.bias is not None:
             y = y + self.bias.to(y.dtype)
         y = apply_activation(y, self.activation)                          # [N, L, O]
@@ -438,7 +444,7 @@ class LocallyConnected1D(Layer):
     def call(self, x):
         win = x.unfold(1, self.k, self.s)                                  # [N, L, D, k]
         win = win.permute(0, 1, 3, 2).reshape(x.shape[0], self.out_steps, -1)
-        y = torch.einsum("nlk,lko->nlo", win, self.weight.to(win.dtype))
+        y = _per_position(win.transpose(0, 1), self.weight.to(win.dtype))
         if self.bias is not None:
             y = y + self.bias.to(y.dtype)
         return apply_activation(y, self.activation)

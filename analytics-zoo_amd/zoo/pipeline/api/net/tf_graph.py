@@ -21,6 +21,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from zoo.ops.bmm import matmul
 from zoo.utils import protobuf as pb
 
 # tensorflow/core/framework/types.proto
@@ -670,7 +671,7 @@ def _matmul(g, node, a, b):
         from zoo import ops
         g.native_calls += 1
         return ops.linear(a.float(), b.t().float().contiguous()).float()
-    return torch.matmul(a, b.to(a.dtype))
+    return matmul(a, b.to(a.dtype))
 
 
 def _batch_matmul(g, node, a, b):
@@ -678,7 +679,7 @@ def _batch_matmul(g, node, a, b):
         a = a.transpose(-1, -2)
     if node.attr.get("adj_y", False):
         b = b.transpose(-1, -2)
-    return torch.matmul(a, b.to(a.dtype))
+    return matmul(a, b.to(a.dtype))
 
 
 def _bias_add(g, node, x, b):

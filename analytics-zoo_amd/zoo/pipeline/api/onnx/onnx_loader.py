@@ -15,6 +15,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from zoo.ops.bmm import matmul
 from zoo.pipeline.api.net import native_lower as NL
 
 from zoo.pipeline.api.net import graph_net as G
@@ -302,7 +303,7 @@ def _gap(x):
 
 
 _OPS = {
-    "Conv": _conv, "Gemm": _gemm, "MatMul": lambda x, a: x[0] @ x[1],
+    "Conv": _conv, "Gemm": _gemm, "MatMul": lambda x, a: matmul(x[0], x[1]),
     "Add": lambda x, a: x[0] + x[1], "Sub": lambda x, a: x[0] - x[1], "Mul": lambda x, a: x[0] * x[1],
     "Div": lambda x, a: x[0] / x[1], "Pow": lambda x, a: x[0] ** x[1], "Neg": lambda x, a: -x[0],
     "Relu": lambda x, a: _act(x[0], "relu", torch.relu), "Sigmoid": lambda x, a: _act(x[0], "sigmoid", torch.sigmoid),

@@ -28,6 +28,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from zoo.ops.bmm import matmul
+
 _NP_TYPES = {"f32": np.float32, "fp32": np.float32, "f16": np.float16, "fp16": np.float16, "f64": np.float64,
              "i64": np.int64, "i32": np.int32, "i8": np.int8, "u8": np.uint8, "i16": np.int16, "u16": np.uint16,
              "boolean": np.bool_, "u1": np.uint8, "bf16": None}
@@ -344,7 +346,7 @@ class OpenVINOModel(nn.Module):
                 from zoo import ops
                 wt = w if tb else w.t()
                 return ops.linear(x.float(), wt.float().contiguous())
-            return torch.matmul(x, w.transpose(-1, -2) if tb else w)
+            return matmul(x, w.transpose(-1, -2) if tb else w)
         if t == "FullyConnected":
             K = int(at.get("out-size"))
             x = a[0].reshape(a[0].shape[0], -1)
