@@ -90,6 +90,7 @@ struct PagedEvictArgs {
   PoolStride ks, vs, ss, ps, sos, pos;
   FastDiv page, vec;
   int B, H, pages, cap, es, budget, recent, most;
+  int over;                  // budget + slack (at most cap): rows of more slots are cut down
   int fused;                 // 1: so little moves that the selecting workgroup does it
   int segs;                  // workgroups to a row, 0: one, its keys in LDS
 };

@@ -898,13 +898,13 @@ ZOO_DEV Counts count_range(int s0, int s1, int K, const Cut& cut, Key key) {
   return c;
 }
 
-// Lists, for the slots s0 .. s1 of one wave, those given up below the budget and those kept behind it, in
+// Lists, for the slots s0 .. s1 of one wave, those given up below the budget K and those kept behind it, in
 // order. `b`: the counts of all slots before s0; `eq_lo`: of the whole row; `masks`: this wave's room in LDS for a bit
 // to each of its slots.
 template <class Key>
-ZOO_DEV void list_range(const PagedEvictArgs& a, const Row& row, int s0, int s1, const Counts& b, int eq_lo,
+ZOO_DEV void list_range(const PagedEvictArgs& a, const Row& row, int s0, int s1, int K, const Counts& b, int eq_lo,
                         const Cut& cut, int* give, int* take, unsigned long long* masks, Key key) {
-  const int lane = threadIdx.x & 63, K = a.budget;
+  const int lane = threadIdx.x & 63;
   const unsigned long long below = (1ull << lane) - 1;
   int equal = b.eq_lo + b.eq_hi;
   int gave = min(s0, K) - b.gt_lo - min(cut.ties, b.eq_lo);
@@ -1009,6 +1009,9 @@ ZOO_DEV void move_rows(const PagedEvictArgs& a, const Row& row, int r, int n, ui
   }
 }
 
+// slots that a row of len may keep: one that is within the slack keeps all of them
+ZOO_DEV int row_budget(const PagedEvictArgs& a, int len) { return len > a.over ? a.budget : max(len, a.budget); }
+
 // One workgroup per row (sequence and kv head), its keys in LDS: a radix selection of the budget-th largest by
 // digits of 11, 11 and 10 bits, then the lists, each wave a stretch of the slots. Bound by its barriers and the latency
 // of its loads: 256 rows of up to 8192 slots 21 us, where reading them takes 2. Rows of up to 2048 slots go to 256
@@ -1023,7 +1026,7 @@ __global__ __launch_bounds__(NT) void paged_evict_select_kernel(const PagedEvict
   __shared__ Counts counts[NT / 64];
   const int b = blockIdx.x / a.H, tid = threadIdx.x, wave = uni(tid >> 6);
   const Row row{a.table + (long)b * a.table_b, a.page, (int)blockIdx.x - b * a.H};
-  const int len = seq_len(a.len, b, a.cap), K = a.budget;
+  const int len = seq_len(a.len, b, a.cap), K = row_budget(a, len);
   const long oldest = (long)a.seen[b] - a.recent;
   const bool digits = len - K > kEvictFew;
   if (tid == 0) s_bad = len < 0;
@@ -1098,7 +1101,7 @@ __global__ __launch_bounds__(NT) void paged_evict_select_kernel(const PagedEvict
   }
   if (gone > 0) cut.ties = eq_all - gone;
   int* give = a.moves + (long)blockIdx.x * 2 * a.most;
-  list_range(a, row, s0, s1, before, eq_lo, cut, give, give + a.most, masks + wave * ((len + NT - 1) / NT), key);
+  list_range(a, row, s0, s1, K, before, eq_lo, cut, give, give + a.most, masks + wave * ((len + NT - 1) / NT), key);
   int gt = 0, eq = 0;   // as many are kept behind the budget as are given up below it
   for (int i = 0; i < NT / 64; ++i) gt += counts[i].gt_hi, eq += counts[i].eq_hi;
   const int n = gt + min(max(cut.ties - eq_lo, 0), eq);
@@ -1122,7 +1125,7 @@ __global__ __launch_bounds__(256) void paged_evict_long_kernel(const PagedEvictA
   __shared__ unsigned long long masks[kEvictSeg / 64];
   const int r = blockIdx.x / a.segs, seg = blockIdx.x - r * a.segs, b = r / a.H, tid = threadIdx.x;
   const Row row{a.table + (long)b * a.table_b, a.page, r - b * a.H};
-  const int len = seq_len(a.len, b, a.cap), K = a.budget;
+  const int len = seq_len(a.len, b, a.cap), K = row_budget(a, len);
   int* flag = a.hist + (long)r * kEvictRow;     // a page of the row is bad
   int* state = flag + 1;                        // [3][3] known bits, left, whole, after each digit
   int* sums = flag + 16;                        // [3][kEvictBins]
@@ -1193,7 +1196,7 @@ __global__ __launch_bounds__(256) void paged_evict_long_kernel(const PagedEvictA
         before = {sum(before.gt_lo), sum(before.eq_lo), sum(before.gt_hi), sum(before.eq_hi)};
         const int eq_lo = sum(all.eq_lo), gt_hi = sum(all.gt_hi), eq_hi = sum(all.eq_hi);
         int* give = a.moves + (long)r * 2 * a.most;
-        list_range(a, row, w0, w1, before, eq_lo, cut, give, give + a.most, masks + wave * (kEvictSeg / 256), key);
+        list_range(a, row, w0, w1, K, before, eq_lo, cut, give, give + a.most, masks + wave * (kEvictSeg / 256), key);
         if (seg == 0 && tid == 0) a.count[r] = gt_hi + min(max(cut.ties - eq_lo, 0), eq_hi);
       }
     }

@@ -3318,13 +3318,14 @@ torch::Tensor paged_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, t
 
 torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scores, torch::Tensor positions,
                           torch::Tensor table, torch::Tensor lengths, torch::Tensor seen, int64_t budget, int64_t recent,
-                          torch::Tensor scores_out, torch::Tensor positions_out) {
+                          torch::Tensor scores_out, torch::Tensor positions_out, int64_t slack) {
   const char* what = "paged_evict";
   const PagedCache c = paged_check(kp, vp, table, lengths, c10::nullopt, what);
   paged_no_grad({&kp, &vp, &scores}, what);
   c10::DeviceGuard guard(kp.device());
   TORCH_CHECK(budget >= 1 && budget <= zoo::kKvMaxSlots, what, ": budget must be from 1 to 2^30");
   TORCH_CHECK(recent >= 0 && recent <= budget, what, ": recent must be from 0 to the budget");
+  TORCH_CHECK(slack >= 0 && slack <= zoo::kKvMaxSlots, what, ": slack must be from 0 to 2^30");
   paged_written(kp, vp, table);
   paged_ints(seen, lengths, "seen", what);
   for (const torch::Tensor* t : {&scores, &scores_out}) paged_side(*t, kp, at::kFloat, "scores", what);
@@ -3352,6 +3353,7 @@ torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scor
   a.page = fast_div((uint32_t)c.page), a.vec = fast_div((uint32_t)vec);
   a.B = c.B, a.H = c.H, a.pages = c.P, a.cap = c.cap, a.es = c.es;
   a.budget = budget, a.recent = recent, a.most = most;
+  a.over = (int)std::min(budget + slack, c.cap);
   a.segs = c.cap > zoo::kEvictHeld ? (c.cap + zoo::kEvictSeg - 1) / zoo::kEvictSeg : 0;
   TORCH_CHECK(rows * std::max(a.segs, 1) < (1LL << 24), what, ": too many heads or slots in the batch");
   // 16-byte pieces of a row's moves that its selecting workgroup moves itself, without a second launch: 384 rows, up to 512

@@ -74,22 +74,23 @@ def paged_append(k, v, k_pages, v_pages, page_table, lengths, counts=None, seen=
 
 
 def paged_evict(k_pages, v_pages, scores, positions, page_table, lengths, seen, budget, recent=0, scores_out=None,
-                positions_out=None):
-    """Cuts every sequence longer than ``budget`` slots down to it, for each kv head by itself: kept are the slots of
+                positions_out=None, slack=0):
+    """Cuts every sequence longer than ``budget + slack`` slots down to ``budget``, for each kv head by itself: kept are the slots of
     the last ``recent`` positions (those >= ``seen[b] - recent``) and then those of the largest score; of equal
     ones the lower slot is kept, and a NaN score counts as the lowest. Kept slots below the budget stay where they
     are; the i-th evicted slot there takes over the i-th kept slot behind the budget, keys, values, score and
-    position, so no more rows move than have to. Returns the new lengths ``min(lengths, budget)`` as a new tensor.
+    position, so no more rows move than have to. A sequence of up to ``budget + slack`` slots keeps them all. Returns the new
+    lengths as a new tensor.
 
     Scores and positions of the kept slots go to ``scores_out`` and ``positions_out``, by default where they were."""
     scores_out = scores if scores_out is None else scores_out
     positions_out = positions if positions_out is None else positions_out
     if k_pages.is_cuda:
         return native().paged_evict(k_pages, v_pages, scores, positions, page_table, lengths, seen, budget, recent,
-                                    scores_out, positions_out)
+                                    scores_out, positions_out, slack)
     _no_grad("paged_evict", k_pages, v_pages, scores)
     return _evict_ref(k_pages, v_pages, scores, positions, page_table, lengths, seen, budget, recent, scores_out,
-                      positions_out)
+                      positions_out, slack)
 
 
 def _capturing(t):
@@ -215,15 +216,18 @@ class PagedKVCache:
         if evict:
             self.evict()
 
+    def _cut(self, n):
+        return self.budget if n > self.budget + self.slack else n
+
     def evict(self):
-        """Cuts the sequences down to the budget if one is longer than budget + slack slots, and gives back the pages
+        """Cuts the sequences that are longer than budget + slack slots down to the budget, and gives back the pages
         that a sequence of budget + slack + 1 slots does not need."""
         if self.budget is None or max(self._slots) <= self.budget + self.slack:
             return
         new = paged_evict(self.k, self.v, self.scores, self.positions, self._table(), self.lengths, self.seen,
-                          self.budget, self.recent)
+                          self.budget, self.recent, slack=self.slack)
         self.lengths.copy_(new)
-        self._slots = [min(n, self.budget) for n in self._slots]
+        self._slots = [self._cut(n) for n in self._slots]
         if _capturing(self.k):
             return
         keep = -(-(self.budget + self.slack + 1) // self.page)
@@ -239,7 +243,7 @@ class PagedKVCache:
         slots = [n + tokens for n in self._slots]      # in use before the eviction
         if any(n > len(own) * self.page for n, own in zip(slots, self._pages)):
             raise RuntimeError("PagedKVCache: the replayed step ran past the pages that were reserved for it")
-        self._slots = [min(n, self.budget) for n in slots] if evicts else slots
+        self._slots = [self._cut(n) for n in slots] if evicts else slots
 
 
 # ---------------------------------------------------------------------------- PyTorch implementation
@@ -327,17 +331,20 @@ def _append_ref(k, v, k_pages, v_pages, page_table, lengths, counts, seen, score
 
 
 def _evict_ref(k_pages, v_pages, scores, positions, page_table, lengths, seen, budget, recent, scores_out,
-               positions_out):
+               positions_out, slack):
     cap = _check(k_pages, v_pages, page_table, lengths)
     if budget < 1 or not 0 <= recent <= budget:
         raise RuntimeError("paged_evict: budget must be at least 1 and recent from 0 to the budget")
+    if slack < 0:
+        raise RuntimeError("paged_evict: slack must not be negative")
     new = lengths.clone()
     for b, at in enumerate(_rows(k_pages, page_table, lengths, cap)):
         if at is None or at[0].numel() == 0:
             continue
         p, r = at
         n = p.numel()
-        new[b] = min(n, budget)
+        keep = budget if n > budget + slack else max(n, budget)
+        new[b] = min(n, keep)
         score, pos = scores[p, :, r], positions[p, :, r]                  # [n, H]
         for h in range(k_pages.shape[1]):
             s = torch.where(torch.isnan(score[:, h]), torch.tensor(-math.inf), score[:, h]).double()
@@ -348,11 +355,11 @@ def _evict_ref(k_pages, v_pages, scores, positions, page_table, lengths, seen, b
             order = torch.argsort(s, descending=True, stable=True)
             order = order[torch.argsort(tier[order], descending=True, stable=True)]
             kept = torch.zeros(n, dtype=torch.bool)
-            kept[order[:budget]] = True
+            kept[order[:keep]] = True
             src = torch.arange(n)
-            hole = (~kept[:budget]).nonzero().flatten()
-            src[hole] = (kept[budget:].nonzero().flatten() + budget)
-            src = src[:min(n, budget)]
+            hole = (~kept[:keep]).nonzero().flatten()
+            src[hole] = (kept[keep:].nonzero().flatten() + keep)
+            src = src[:min(n, keep)]
             m = src.numel()
             for pool, out in ((k_pages, k_pages), (v_pages, v_pages), (scores, scores_out), (positions, positions_out)):
                 out[p[:m], h, r[:m]] = pool[p[src], h, r[src]]

@@ -627,3 +627,45 @@ def test_bad_pages_leave_the_gathered_weights(dev, H, G, D, page, dtype, lengths
     assert all(bool(torch.isnan(out[p, 0, r])) for p, r in rows[3])
     assert all(torch.equal(out[p, :, r], good[p, :, r]) for b in range(3) for p, r in rows[b])
     assert all(torch.equal(out[p, 1:, r], good[p, 1:, r]) for p, r in rows[3])
+
+
+# ---------------------------------------------------------------------------- slack
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("H,D,page,dtype,lengths,budget,slack", [
+    (2, 64, 16, BF, [100, 0, 50, 51, 58, 59, 1], 50, 8), (1, 8, 7, FL, [60, 20, 13, 14], 1, 13),
+    (2, 16, 33, FL, [1500, 1100, 1024, 1025], 700, 324), (1, 8, 128, BF, [2500, 3000], 2048, 2 ** 30),
+    (2, 8, 64, FL, [20000, 18000, 17999, 5, 300], 17000, 999),        # rows shared out
+])
+def test_evict_with_slack(dev, H, D, page, dtype, lengths, budget, slack):
+    """Rows of up to budget + slack slots keep them all, and their scores and positions go to the new pools as well."""
+    _, k, v, table, n = make(len(lengths), H, 1, D, page, lengths, dtype, dev, junk=2.0)
+    g = torch.Generator().manual_seed(5)
+    scores = torch.rand(k.shape[:3], generator=g).to(dev)
+    positions = torch.randint(0, 10 ** 6, k.shape[:3], generator=g, dtype=torch.int32).to(dev)
+    seen = torch.full_like(n, 10 ** 6)
+    cut = [b for b, m in enumerate(lengths) if m > budget + slack]
+    kept = [min(m, budget) if b in cut else m for b, m in enumerate(lengths)]
+    want = evict_by_definition((k, v, scores, positions), table[cut], [lengths[b] for b in cut], [10 ** 6] * len(cut), budget, 0)
+    k2, v2 = k.clone(), v.clone()
+    so, po = torch.full_like(scores, -5.0), torch.full_like(positions, -5)
+    got = paged_evict(k2, v2, scores, positions, table, n, seen, budget, scores_out=so, positions_out=po, slack=slack)
+    assert got.tolist() == kept
+    assert torch.equal(k2, want[0]) and torch.equal(v2, want[1])
+    used = torch.zeros(k.shape[:3], dtype=torch.bool)
+    for b, m in enumerate(kept):
+        s = torch.arange(m)
+        used[table.cpu()[b, s // page].long(), :, s % page] = True
+    used = used.to(dev)
+    assert torch.equal(so[used], want[2][used]) and torch.equal(po[used], want[3][used])
+    assert (so[~used] == -5.0).all() and (po[~used] == -5).all()
+    assert paged_evict(k, v, scores, positions, table, n, seen, budget, slack=slack).tolist() == kept
+    for x, y in zip((k, v, scores, positions), want):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+def test_slack_refusals(dev):
+    _, k, v, table, n = make(2, 2, 2, 16, 8, [9, 5], BF, dev)
+    s, p = torch.zeros(k.shape[:3]).to(dev), torch.zeros(k.shape[:3]).int().to(dev)
+    with pytest.raises(RuntimeError, match="slack"):
+        paged_evict(k, v, s, p, table, n, n, 4, slack=-1)
