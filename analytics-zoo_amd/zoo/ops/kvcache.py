@@ -202,7 +202,7 @@ class PagedKVCache:
 
     def advance(self, tokens, lengths, rows=None, evict=True):
         """Ends a step that gave the rows ``tokens`` tokens (a number, or one for each row): ``lengths`` are in use now,
-        less what eviction takes."""
+        less what eviction takes from these rows."""
         r = range(self.batch) if rows is None else rows
         tokens = [tokens] * len(r) if isinstance(tokens, int) else list(tokens)
         if rows is None:
@@ -214,28 +214,31 @@ class PagedKVCache:
         for x, t in zip(r, tokens):
             self._slots[x] += t
         if evict:
-            self.evict()
+            self.evict(rows)
 
     def _cut(self, n):
         return self.budget if n > self.budget + self.slack else n
 
-    def evict(self):
-        """Cuts the sequences that are longer than budget + slack slots down to the budget, and gives back the pages
-        that a sequence of budget + slack + 1 slots does not need."""
-        if self.budget is None or max(self._slots) <= self.budget + self.slack:
+    def evict(self, rows=None):
+        """Cuts the sequences (all, or the ``rows``, a list) that are longer than budget + slack slots down to the
+        budget, and gives back the pages that a sequence of budget + slack + 1 slots does not need."""
+        r = range(self.batch) if rows is None else rows
+        if self.budget is None or max((self._slots[x] for x in r), default=0) <= self.budget + self.slack:
             return
-        new = paged_evict(self.k, self.v, self.scores, self.positions, self._table(), self.lengths, self.seen,
-                          self.budget, self.recent, slack=self.slack)
-        self.lengths.copy_(new)
-        self._slots = [self._cut(n) for n in self._slots]
+        at = slice(None) if rows is None else rows
+        self.lengths[at] = paged_evict(self.k, self.v, self.scores, self.positions, self._table()[at], self.lengths[at],
+                                       self.seen[at], self.budget, self.recent, slack=self.slack)
+        for x in r:
+            self._slots[x] = self._cut(self._slots[x])
         if _capturing(self.k):
             return
         keep = -(-(self.budget + self.slack + 1) // self.page)
-        for r, own in enumerate(self._pages):
+        for x in r:
+            own = self._pages[x]
             if len(own) > keep:
                 self._free += own[keep:]
                 del own[keep:]
-                self.page_table[r, keep:] = -1
+                self.page_table[x, keep:] = -1
 
     def replayed(self, tokens=1, evicts=False):
         """Tells the host's book that a captured step, which gave every row ``tokens`` tokens and ended with an eviction

@@ -426,3 +426,25 @@ def test_a_rows_eviction_is_its_own(dev, slack):
             if dev == "cpu":    # products of other batch sizes round otherwise on the GPU, which may turn a close choice
                 near(y[b], y1[0], dev)
                 assert held[b] == held1[0]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_a_row_that_waits_is_not_cut(dev):
+    """A prompt past the budget has gathered no weight before its first step: steps of other rows leave it whole."""
+    t = layer(dev, blocks=1)
+    tok, pos = ids(3, 40, dev)
+    c = t.init_cache(3, max_length=40, page=4, budget=8, recent=2)
+    t.prefill([tok[:, :20], pos[:, :20]], c, counts=[20, 8, 3])
+    own = list(c._pages[0])
+    t.decode([tok[1:, 20], pos[1:, 20]], c, rows=[1, 2])
+    assert c._slots == [20, 8, 4] == c.lengths.tolist() and c.seen.tolist() == [20, 9, 4] and c._pages[0] == own
+    t.decode([tok[[2, 1], 21], pos[[2, 1], 21]], c, rows=[2, 1])
+    assert c._slots == [20, 8, 5] == c.lengths.tolist() and c.seen.tolist() == [20, 10, 5]
+    where = [(int(c.page_table[0, s // 4]), s % 4) for s in range(20)]
+    assert [int(c.positions[p, 0, r]) for p, r in where] == list(range(20))
+    t.decode([tok[:1, 20], pos[:1, 20]], c, rows=[0])
+    assert c._slots == [8, 8, 5] == c.lengths.tolist() and len(c._pages[0]) == 3
+    used = [p for pages in c._pages for p in pages]
+    assert len(used) == len(set(used)) and not set(used) & set(c._free)
+    c.evict()
+    assert c._slots == [8, 8, 5]
