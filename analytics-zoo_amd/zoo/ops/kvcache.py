@@ -30,6 +30,7 @@ Extends TransformerLayer (Zs/pipeline/api/keras/layers/TransformerLayer.scala:13
 reference only evaluates over whole sequences.
 """
 import math
+import operator
 
 import torch
 
@@ -152,10 +153,29 @@ class PagedKVCache:
         return (self.k[:, h], self.v[:, h], None if self.scores is None else self.scores[:, h],
                 None if self.positions is None else self.positions[:, h])
 
+    def rows(self, rows=None):
+        """Row numbers as a list, those from the end as numbers from 0; all of them for None. A row may come once."""
+        if rows is None:
+            return list(range(self.batch))
+        rows = [operator.index(r) for r in rows]
+        if not all(-self.batch <= r < self.batch for r in rows):
+            raise IndexError("PagedKVCache: rows from 0 to %d" % (self.batch - 1))
+        rows = [r % self.batch for r in rows]
+        if len(set(rows)) != len(rows):
+            raise ValueError("PagedKVCache: a row is named twice")
+        return rows
+
+    @staticmethod
+    def _tokens(tokens, rows):
+        tokens = [tokens] * len(rows) if isinstance(tokens, int) else [int(t) for t in tokens]
+        if len(tokens) != len(rows) or any(t < 0 for t in tokens):
+            raise ValueError("PagedKVCache: a number of tokens, not negative, for each row")
+        return tokens
+
     def reserve(self, tokens, rows=None):
         """Takes the pages that ``tokens`` (a number, or one for each row) more tokens of the rows need."""
-        rows = range(self.batch) if rows is None else rows
-        tokens = [tokens] * len(rows) if isinstance(tokens, int) else list(tokens)
+        rows = self.rows(rows)
+        tokens = self._tokens(tokens, rows)
         want = [-(-(self._slots[r] + t) // self.page) for r, t in zip(rows, tokens)]
         if any(self._slots[r] + t > self.max_length for r, t in zip(rows, tokens)):
             raise RuntimeError("PagedKVCache: a sequence would be longer than max_length = %d slots" % self.max_length)
@@ -187,8 +207,8 @@ class PagedKVCache:
         return self.page_table[:, :max(1, width)]
 
     def append(self, i, k, v, counts=None, rows=None):
-        """``paged_append`` to layer ``i`` of all rows, or of the ``rows`` (int64 [n] on the device); returns the new
-        lengths, which :meth:`advance` makes the cache's."""
+        """``paged_append`` to layer ``i`` of all rows, or of the ``rows`` (int64 [n] on the device, each once); returns the
+        new lengths, which :meth:`advance` makes the cache's."""
         kp, vp, scores, positions = self.layer(i)
         at = slice(None) if rows is None else rows
         return paged_append(k, v, kp, vp, self._table()[at], self.lengths[at], counts=counts, seen=self.seen[at],
@@ -203,14 +223,14 @@ class PagedKVCache:
     def advance(self, tokens, lengths, rows=None, evict=True):
         """Ends a step that gave the rows ``tokens`` tokens (a number, or one for each row): ``lengths`` are in use now,
         less what eviction takes from these rows."""
-        r = range(self.batch) if rows is None else rows
-        tokens = [tokens] * len(r) if isinstance(tokens, int) else list(tokens)
+        r = self.rows(rows)
+        tokens = self._tokens(tokens, r)
         if rows is None:
             self.seen += lengths - self.lengths
             self.lengths.copy_(lengths)
         else:
-            self.seen[rows] += lengths - self.lengths[rows]
-            self.lengths[rows] = lengths
+            self.seen[r] += lengths - self.lengths[r]
+            self.lengths[r] = lengths
         for x, t in zip(r, tokens):
             self._slots[x] += t
         if evict:
@@ -222,10 +242,10 @@ class PagedKVCache:
     def evict(self, rows=None):
         """Cuts the sequences (all, or the ``rows``, a list) that are longer than budget + slack slots down to the
         budget, and gives back the pages that a sequence of budget + slack + 1 slots does not need."""
-        r = range(self.batch) if rows is None else rows
+        r = self.rows(rows)
         if self.budget is None or max((self._slots[x] for x in r), default=0) <= self.budget + self.slack:
             return
-        at = slice(None) if rows is None else rows
+        at = slice(None) if rows is None else r
         self.lengths[at] = paged_evict(self.k, self.v, self.scores, self.positions, self._table()[at], self.lengths[at],
                                        self.seen[at], self.budget, self.recent, slack=self.slack)
         for x in r:

@@ -198,11 +198,11 @@ class TransformerLayer(Layer):
         the rest is padding behind them. Returns the sequence output [n, T, hidden], as the layer's own call
         does."""
         n, T = xs[0].shape
-        at = list(range(cache.batch)) if rows is None else list(rows)
+        at = cache.rows(rows)
         counts = [T] * n if counts is None else [int(c) for c in counts]
         if n == 0 or T == 0:
             raise ValueError("prefill: no prompts, or none with a token")
-        if len(at) != n or len(counts) != n or len(set(at)) != n:
+        if len(at) != n or len(counts) != n:
             raise ValueError("prefill: a row of the cache and a count for each prompt")
         if not all(0 <= c <= T for c in counts):
             raise ValueError("prefill: counts from 0 to the prompts' length")
@@ -225,11 +225,12 @@ class TransformerLayer(Layer):
     def decode(self, xs, cache, rows=None):
         """One token of every row of ``cache``, or of the rows ``rows`` (a list of numbers): ``xs`` = [token_ids,
         position_ids] ([n]). Returns the sequence output of these tokens [n, hidden]."""
-        n = cache.batch if rows is None else len(rows)
-        if n == 0 or xs[0].dim() != 1 or xs[0].shape[0] != n or (rows is not None and len(set(rows)) != n):
+        at = cache.rows(rows)
+        n = len(at)
+        if n == 0 or xs[0].dim() != 1 or xs[0].shape[0] != n:
             raise ValueError("decode: one token for each row of the cache")
-        cache.reserve(1, rows)
-        sub = None if rows is None else torch.tensor(list(rows)).to(cache.k.device)
+        cache.reserve(1, None if rows is None else at)
+        sub = None if rows is None else torch.tensor(at).to(cache.k.device)
         new = []
 
         def cached(i, blk, qkv):
@@ -237,7 +238,7 @@ class TransformerLayer(Layer):
             new[:] = [cache.append(i, k, v, rows=sub)]
             return cache.attend(i, q[:, 0], new[0], rows=sub).reshape(n, 1, -1).to(qkv.dtype)
         x = self._cached_run(self._embed([t.unsqueeze(1) for t in xs]), cached)
-        cache.advance(1, new[0], rows)
+        cache.advance(1, new[0], None if rows is None else at)
         return x[:, 0]
 
 

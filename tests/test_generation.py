@@ -448,3 +448,26 @@ def test_a_row_that_waits_is_not_cut(dev):
     assert len(used) == len(set(used)) and not set(used) & set(c._free)
     c.evict()
     assert c._slots == [8, 8, 5]
+
+
+def test_rows_are_counted_from_either_end_and_named_once():
+    t = layer("cpu")
+    tok, pos = ids(3, 10, "cpu")
+    a, b = t.init_cache(3, page=4), t.init_cache(3, page=4)
+    for c, rows in ((a, [2, 0]), (b, [-1, 0])):
+        t.prefill([tok[:2], pos[:2]], c, rows=rows)
+        y = t.decode([tok[:2, 0], pos[:2, 0]], c, rows=rows)
+        assert c._slots == [11, 0, 11] == c.lengths.tolist() == c.seen.tolist()
+    assert torch.equal(a.page_table, b.page_table) and torch.equal(a.k, b.k) and torch.isfinite(y).all()
+    free = list(b._free)
+    for call in (lambda: t.decode([tok[:2, 0], pos[:2, 0]], b, rows=[2, -1]),
+                 lambda: t.prefill([tok[:2], pos[:2]], b, rows=[1, -2]),
+                 lambda: b.reserve(3, [1, -2]), lambda: b.reserve([1, 2], [1]), lambda: b.reserve([1, 1]),
+                 lambda: b.reserve([1, -1, 1]), lambda: b.reserve(-1),
+                 lambda: b.advance([1, 1], b.lengths), lambda: b.advance(1, b.lengths[:2], [0, 0])):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: t.decode([tok[:1, 0], pos[:1, 0]], b, rows=[3]), lambda: b.reserve(1, [-4])):
+        with pytest.raises(IndexError):
+            call()
+    assert b._slots == [11, 0, 11] == b.lengths.tolist() == b.seen.tolist() and b._free == free
