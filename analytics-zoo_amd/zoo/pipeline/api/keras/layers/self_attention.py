@@ -176,11 +176,13 @@ class TransformerLayer(Layer):
         return ops.PagedKVCache(self.n_block, batch, max_length, self.n_head, self.hidden // self.n_head, page=page,
                                 pages=pages, budget=budget, recent=recent, slack=slack, device=w.device)
 
-    def _cached_run(self, x, cached):
+    def _cached_check(self):
         if self.bidirectional:
             raise RuntimeError("a bidirectional TransformerLayer sees the whole sequence: it cannot go token by token")
         if self.training:
             raise RuntimeError("generation with a cache needs eval(): dropout would act on it")
+
+    def _cached_run(self, x, cached):
         for i, blk in enumerate(self.blocks):
             x = blk(x, None, causal=True, cached=lambda qkv, i=i, blk=blk: cached(i, blk, qkv))
         return x
@@ -208,6 +210,7 @@ class TransformerLayer(Layer):
             raise ValueError("prefill: counts from 0 to the prompts' length")
         if any(cache._slots[r] for r in at):
             raise RuntimeError("prefill: the cache's rows are in use: release them first")
+        self._cached_check()
         cache.reserve(counts, at)
         real = torch.tensor(counts, dtype=torch.int32).to(cache.k.device)
         sub = None if rows is None else torch.tensor(at).to(cache.k.device)
@@ -229,6 +232,7 @@ class TransformerLayer(Layer):
         n = len(at)
         if n == 0 or xs[0].dim() != 1 or xs[0].shape[0] != n:
             raise ValueError("decode: one token for each row of the cache")
+        self._cached_check()
         cache.reserve(1, None if rows is None else at)
         sub = None if rows is None else torch.tensor(at).to(cache.k.device)
         new = []

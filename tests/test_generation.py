@@ -471,3 +471,16 @@ def test_rows_are_counted_from_either_end_and_named_once():
         with pytest.raises(IndexError):
             call()
     assert b._slots == [11, 0, 11] == b.lengths.tolist() == b.seen.tolist() and b._free == free
+
+
+def test_a_refused_prompt_takes_no_pages():
+    t = layer("cpu")
+    tok, pos = ids(2, 10, "cpu")
+    both = TransformerLayer.init(vocab=80, seq_len=8, n_block=1, hidden_size=16, n_head=2, bidirectional=True).eval()
+    c, d = t.train().init_cache(2, page=4), both.init_cache(2, max_length=12, page=4)
+    for run, cache, x in ((t, c, [tok, pos]), (both, d, [tok % 8, pos % 8])):
+        free = list(cache._free)
+        for call in (lambda: run.prefill(x, cache), lambda: run.decode([x[0][:, 0], x[1][:, 0]], cache)):
+            with pytest.raises(RuntimeError):
+                call()
+        assert cache._free == free and not (cache.page_table >= 0).any()
