@@ -109,7 +109,7 @@ class PagedKVCache:
 
     A step of every layer: :meth:`append`, :meth:`attend` per layer, then :meth:`advance`.
 
-    Inside a captured hipGraph no page can be taken. So ``reserve`` what a step needs before the capture and before each
+    A captured hipGraph can hold steps of all rows, and takes no pages. So ``reserve`` what a step needs before the capture and before each
     replay (which raises where a replay could not be carried out), and tell the host's book about the replay with
     :meth:`replayed` after it. Between replays rows may be released and filled again. A captured step is laid out for rows
     of ``max_length`` slots, or of all ``pages``: that bounds its workspace, so make it no larger than needed."""
@@ -165,6 +165,11 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: a row is named twice")
         return rows
 
+    def not_captured(self, what):
+        """Raises where a hipGraph is being captured: ``what`` needs copies from the host, which a replay could not repeat."""
+        if _capturing(self.k):
+            raise RuntimeError("PagedKVCache: %s cannot be captured" % what)
+
     @staticmethod
     def _tokens(tokens, rows):
         tokens = [tokens] * len(rows) if isinstance(tokens, int) else [int(t) for t in tokens]
@@ -191,6 +196,7 @@ class PagedKVCache:
 
     def release(self, rows=None):
         """Empties rows and gives their pages back."""
+        self.not_captured("releasing rows")
         for r in range(self.batch) if rows is None else rows:
             self._free += self._pages[r]
             self._pages[r], self._slots[r] = [], 0
@@ -225,6 +231,8 @@ class PagedKVCache:
         less what eviction takes from these rows."""
         r = self.rows(rows)
         tokens = self._tokens(tokens, r)
+        if rows is not None:
+            self.not_captured("a step of some rows")
         if rows is None:
             self.seen += lengths - self.lengths
             self.lengths.copy_(lengths)
@@ -243,6 +251,8 @@ class PagedKVCache:
         """Cuts the sequences (all, or the ``rows``, a list) that are longer than budget + slack slots down to the
         budget, and gives back the pages that a sequence of budget + slack + 1 slots does not need."""
         r = self.rows(rows)
+        if rows is not None:
+            self.not_captured("an eviction from some rows")
         if self.budget is None or max((self._slots[x] for x in r), default=0) <= self.budget + self.slack:
             return
         at = slice(None) if rows is None else r

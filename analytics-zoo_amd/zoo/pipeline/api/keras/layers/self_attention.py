@@ -211,6 +211,7 @@ class TransformerLayer(Layer):
         if any(cache._slots[r] for r in at):
             raise RuntimeError("prefill: the cache's rows are in use: release them first")
         self._cached_check()
+        cache.not_captured("a prompt")
         cache.reserve(counts, at)
         real = torch.tensor(counts, dtype=torch.int32).to(cache.k.device)
         sub = None if rows is None else torch.tensor(at).to(cache.k.device)
@@ -233,6 +234,8 @@ class TransformerLayer(Layer):
         if n == 0 or xs[0].dim() != 1 or xs[0].shape[0] != n:
             raise ValueError("decode: one token for each row of the cache")
         self._cached_check()
+        if rows is not None:
+            cache.not_captured("a step of some rows")
         cache.reserve(1, None if rows is None else at)
         sub = None if rows is None else torch.tensor(at).to(cache.k.device)
         new = []

@@ -484,3 +484,20 @@ def test_a_refused_prompt_takes_no_pages():
             with pytest.raises(RuntimeError):
                 call()
         assert cache._free == free and not (cache.page_table >= 0).any()
+
+
+def test_a_capture_takes_all_rows_one_token_each(monkeypatch):
+    """Row numbers and counts come from the host: a captured step cannot take them, and says so before it records."""
+    import zoo.ops.kvcache as kvcache
+    t = layer("cpu")
+    tok, pos = ids(2, 10, "cpu")
+    c = t.init_cache(2, max_length=12, page=4)
+    c.reserve(2)
+    monkeypatch.setattr(kvcache, "_capturing", lambda x: True)
+    for call in (lambda: t.decode([tok[:1, 0], pos[:1, 0]], c, rows=[1]), lambda: t.prefill([tok[:, :2], pos[:, :2]], c),
+                 lambda: c.evict([0]), lambda: c.advance(1, c.lengths[:1] + 1, [0]), lambda: c.release([0])):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            call()
+    assert c._slots == [0, 0] == c.lengths.tolist() and [len(p) for p in c._pages] == [1, 1]
+    t.decode([tok[:, 0], pos[:, 0]], c)
+    assert c._slots == [1, 1]
