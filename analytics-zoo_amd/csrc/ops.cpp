@@ -3214,6 +3214,7 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
     paged_no_grad({&*scores}, what);
     if (!scores_out.has_value()) scores_out = scores;
     paged_side(*scores_out, kp, at::kFloat, "scores_out", what);
+    paged_no_grad({&*scores_out}, what);
     at::assert_no_internal_overlap(*scores_out);
     at::assert_no_partial_overlap(*scores_out, *scores);
   }
@@ -3291,6 +3292,7 @@ torch::Tensor paged_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, t
   if (seen.has_value()) paged_ints(*seen, lengths, "seen", what);
   if (scores.has_value()) {
     paged_side(*scores, kp, at::kFloat, "scores", what);
+    paged_no_grad({&*scores}, what);
     at::assert_no_internal_overlap(*scores);
   }
   if (positions.has_value()) {
@@ -3321,7 +3323,7 @@ torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scor
                           torch::Tensor scores_out, torch::Tensor positions_out, int64_t slack) {
   const char* what = "paged_evict";
   const PagedCache c = paged_check(kp, vp, table, lengths, c10::nullopt, what);
-  paged_no_grad({&kp, &vp, &scores}, what);
+  paged_no_grad({&kp, &vp, &scores, &scores_out}, what);
   c10::DeviceGuard guard(kp.device());
   TORCH_CHECK(budget >= 1 && budget <= zoo::kKvMaxSlots, what, ": budget must be from 1 to 2^30");
   TORCH_CHECK(recent >= 0 && recent <= budget, what, ": recent must be from 0 to the budget");

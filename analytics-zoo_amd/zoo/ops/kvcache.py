@@ -57,7 +57,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, scores
         scale = 1.0 / math.sqrt(q.shape[-1])
     if k_pages.is_cuda:
         return native().paged_attention(q, k_pages, v_pages, page_table, lengths, scale, scores, scores_out, max_length)
-    _no_grad("paged_attention", q, k_pages, v_pages, scores)
+    _no_grad("paged_attention", q, k_pages, v_pages, scores, scores_out)
     return _attention_ref(q, k_pages, v_pages, page_table, lengths, scale, scores, scores_out, max_length)
 
 
@@ -70,7 +70,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, lengths, counts=None, seen=
     sequence is then longer than its table and its attention NaN."""
     if k_pages.is_cuda:
         return native().paged_append(k, v, k_pages, v_pages, page_table, lengths, counts, seen, scores, positions)
-    _no_grad("paged_append", k, v, k_pages, v_pages)
+    _no_grad("paged_append", k, v, k_pages, v_pages, scores)
     return _append_ref(k, v, k_pages, v_pages, page_table, lengths, counts, seen, scores, positions)
 
 
@@ -89,7 +89,7 @@ def paged_evict(k_pages, v_pages, scores, positions, page_table, lengths, seen, 
     if k_pages.is_cuda:
         return native().paged_evict(k_pages, v_pages, scores, positions, page_table, lengths, seen, budget, recent,
                                     scores_out, positions_out, slack)
-    _no_grad("paged_evict", k_pages, v_pages, scores)
+    _no_grad("paged_evict", k_pages, v_pages, scores, scores_out)
     return _evict_ref(k_pages, v_pages, scores, positions, page_table, lengths, seen, budget, recent, scores_out,
                       positions_out, slack)
 

@@ -669,3 +669,20 @@ def test_slack_refusals(dev):
     s, p = torch.zeros(k.shape[:3]).to(dev), torch.zeros(k.shape[:3]).int().to(dev)
     with pytest.raises(RuntimeError, match="slack"):
         paged_evict(k, v, s, p, table, n, n, 4, slack=-1)
+
+
+# ---------------------------------------------------------------------------- what is written
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+def test_written_pools_that_require_gradients_are_refused(dev):
+    q, k, v, table, n = make(2, 2, 2, 16, 8, [9, 5], FL, dev)
+    s, p = torch.zeros(k.shape[:3]).to(dev), torch.zeros(k.shape[:3]).int().to(dev)
+    x = torch.zeros(2, 1, 2, 16).to(dev)
+    leaf = torch.zeros_like(s).requires_grad_()
+    for call in (lambda: paged_attention(q, k, v, table, n, scores=s, scores_out=leaf),
+                 lambda: paged_append(x, x, k, v, table, n, scores=leaf),
+                 lambda: paged_evict(k, v, s, p, table, n, n, 4, scores_out=leaf)):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+    with torch.no_grad():
+        paged_attention(q, k, v, table, n, scores=s, scores_out=leaf)
+    assert leaf.detach().any()
