@@ -3186,8 +3186,16 @@ void paged_written(const torch::Tensor& kp, const torch::Tensor& vp, const torch
   at::assert_no_internal_overlap(kp);
   at::assert_no_internal_overlap(vp);
   at::assert_no_partial_overlap(kp, vp);
-  TORCH_CHECK(at::get_overlap_status(kp, vp) != at::MemOverlapStatus::Full || kp.numel() == 0,
-              "k_pages and v_pages are the same memory");
+  TORCH_CHECK(kp.data_ptr() != vp.data_ptr() || kp.numel() == 0, "k_pages and v_pages are the same memory");
+}
+
+// a pool that is written from another one: that one itself, in the same layout, or memory apart from it
+void paged_out(const torch::Tensor& out, const torch::Tensor& in, const char* what) {
+  at::assert_no_internal_overlap(out);
+  at::assert_no_partial_overlap(out, in);
+  if (out.data_ptr() != in.data_ptr() || out.numel() == 0) return;
+  for (int64_t i = 0; i < out.dim(); ++i)
+    TORCH_CHECK(out.size(i) == 1 || out.stride(i) == in.stride(i), what, ": a pool is written over itself in another layout");
 }
 
 torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor vp, torch::Tensor table,
@@ -3215,8 +3223,7 @@ torch::Tensor paged_attention(torch::Tensor q, torch::Tensor kp, torch::Tensor v
     if (!scores_out.has_value()) scores_out = scores;
     paged_side(*scores_out, kp, at::kFloat, "scores_out", what);
     paged_no_grad({&*scores_out}, what);
-    at::assert_no_internal_overlap(*scores_out);
-    at::assert_no_partial_overlap(*scores_out, *scores);
+    paged_out(*scores_out, *scores, what);
   }
   auto o = torch::empty({c.B, c.H * G, c.D}, q.options());
   if (o.numel() == 0) return o;
@@ -3332,10 +3339,8 @@ torch::Tensor paged_evict(torch::Tensor kp, torch::Tensor vp, torch::Tensor scor
   paged_ints(seen, lengths, "seen", what);
   for (const torch::Tensor* t : {&scores, &scores_out}) paged_side(*t, kp, at::kFloat, "scores", what);
   for (const torch::Tensor* t : {&positions, &positions_out}) paged_side(*t, kp, at::kInt, "positions", what);
-  at::assert_no_internal_overlap(scores_out);
-  at::assert_no_internal_overlap(positions_out);
-  at::assert_no_partial_overlap(scores_out, scores);
-  at::assert_no_partial_overlap(positions_out, positions);
+  paged_out(scores_out, scores, what);
+  paged_out(positions_out, positions, what);
   auto len_out = torch::empty({c.B}, lengths.options());
   if (c.B == 0) return len_out;
   const int64_t vec = c.D * c.es / 16, rows = c.B * c.H;

@@ -295,6 +295,17 @@ def _check(k_pages, v_pages, page_table, lengths, max_length=None):
     return cap if max_length is None else min(cap, max_length)
 
 
+def _apart(k_pages, v_pages):
+    if k_pages.numel() and k_pages.data_ptr() == v_pages.data_ptr():
+        raise RuntimeError("paged cache: k_pages and v_pages are the same memory")
+
+
+def _out(out, pool):
+    if out.numel() and out.data_ptr() == pool.data_ptr() and \
+            any(n > 1 and x != y for n, x, y in zip(out.shape, out.stride(), pool.stride())):
+        raise RuntimeError("paged cache: a pool is written over itself in another layout")
+
+
 def _rows(k_pages, page_table, lengths, cap):
     """For each sequence: its pages and rows in slot order, or None where length or table are bad."""
     out = []
@@ -320,6 +331,8 @@ def _attention_ref(q, k_pages, v_pages, page_table, lengths, scale, scores, scor
     if scores is None and scores_out is not None:
         raise RuntimeError("paged_attention: scores_out without scores")
     scores_out = scores if scores_out is None else scores_out
+    if scores is not None:
+        _out(scores_out, scores)
     o = torch.zeros(B, Hq, D, dtype=q.dtype)
     for b, at in enumerate(_rows(k_pages, page_table, lengths, cap)):
         if at is None:
@@ -342,6 +355,7 @@ def _append_ref(k, v, k_pages, v_pages, page_table, lengths, counts, seen, score
     if v.shape != k.shape or (H, D) != (k_pages.shape[1], k_pages.shape[3]) or B != page_table.shape[0] \
             or k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
         raise RuntimeError("paged_append: k and v must be [batch, tokens, kv_heads, dim] of the cache's type")
+    _apart(k_pages, v_pages)
     new = lengths.clone()
     page = k_pages.shape[2]
     for b, n in enumerate(lengths.tolist()):
@@ -370,6 +384,9 @@ def _evict_ref(k_pages, v_pages, scores, positions, page_table, lengths, seen, b
         raise RuntimeError("paged_evict: budget must be at least 1 and recent from 0 to the budget")
     if slack < 0:
         raise RuntimeError("paged_evict: slack must not be negative")
+    _apart(k_pages, v_pages)
+    _out(scores_out, scores)
+    _out(positions_out, positions)
     new = lengths.clone()
     for b, at in enumerate(_rows(k_pages, page_table, lengths, cap)):
         if at is None or at[0].numel() == 0:

@@ -686,3 +686,35 @@ def test_written_pools_that_require_gradients_are_refused(dev):
     with torch.no_grad():
         paged_attention(q, k, v, table, n, scores=s, scores_out=leaf)
     assert leaf.detach().any()
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+def test_pools_in_one_place_are_refused(dev):
+    """Keys and values, or scores and where they go, that are the same memory in views which are not dense or are laid
+    out in another order. Views that lie side by side in one tensor are fine."""
+    q, k, v, table, n = make(2, 2, 2, 16, 8, [9, 5], FL, dev, junk=0.0)
+    P = k.shape[0]
+    s, p = torch.zeros(P, 2, 8).to(dev), torch.zeros(P, 2, 8).int().to(dev)
+    x = torch.ones(2, 1, 2, 16).to(dev)
+    layers = torch.zeros(P, 4, 8, 16).to(dev)
+    one = layers[:, 1:3]
+    for call in (lambda: paged_append(x, x, one, layers[:, 1:3], table, n),
+                 lambda: paged_evict(one, layers[:, 1:3], s, p, table, n, n, 4)):
+        with pytest.raises(RuntimeError):
+            call()
+    square = torch.rand(P, 8, 8).to(dev)          # 8 heads, pages of 8: the transposed view has the same sizes
+    k8, v8 = (torch.zeros(P, 8, 8, 16).to(dev) for _ in range(2))
+    p8 = torch.zeros(P, 8, 8).int().to(dev)
+    q8 = torch.zeros(2, 8, 16).to(dev)
+    for call in (lambda: paged_attention(q8, k8, v8, table, n, scores=square, scores_out=square.transpose(1, 2)),
+                 lambda: paged_evict(k8, v8, square, p8, table, n, n, 4, scores_out=square.transpose(1, 2)),
+                 lambda: paged_evict(k8, v8, square, p8, table, n, n, 4, positions_out=p8.transpose(1, 2))):
+        with pytest.raises(RuntimeError):
+            call()
+    assert not layers.any()
+    paged_append(x, x, layers[:, :2], layers[:, 2:], table, n)
+    assert layers.any()
+    both = torch.zeros(P, 2, 2, 8).to(dev)
+    paged_attention(q, k, v, table, n, scores=both[:, 0], scores_out=both[:, 1])
+    paged_attention(q, k, v, table, n, scores=both[:, 0], scores_out=both[:, 0])
+    assert both[:, 0].any()
