@@ -501,3 +501,58 @@ def test_a_capture_takes_all_rows_one_token_each(monkeypatch):
     assert c._slots == [0, 0] == c.lengths.tolist() and [len(p) for p in c._pages] == [1, 1]
     t.decode([tok[:, 0], pos[:, 0]], c)
     assert c._slots == [1, 1]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("D,page,budget", [(16, 8, None), (64, 16, None), (128, 64, None), (128, 7, 30), (64, 16, 24)])
+def test_attention_over_the_cache_against_64_bits(dev, D, page, budget):
+    """A layer's part of the pools as prompts, steps of all and of some rows, and evictions leave it: attention agrees with
+    the definition to the tolerance of the operator, and a missing token or even weights would not."""
+    from test_kvcache import close, define
+    H, layers, rows = 3, 2, [0, 2]
+    c = PagedKVCache(layers, 3, 60, H, D, page=page, budget=budget, recent=4 if budget else None, device=dev)
+    g = torch.Generator().manual_seed(7)
+    kv = torch.randn(layers, 3, 40, 2, H, D, generator=g).to(c.k.dtype).to(dev)
+    q = (torch.randn(layers, 3, 40, H, D, generator=g) * 1.5).to(c.k.dtype).to(dev)
+    fed = [[], [], []]          # tokens of each row, in order
+
+    def step(take, counts, at=None):
+        """Appends tokens take .. to the rows and attends with the last one."""
+        every = list(range(3)) if at is None else at
+        sub = None if at is None else torch.tensor(at, device=dev)
+        c.reserve(counts, at)
+        n = torch.tensor(counts, dtype=torch.int32, device=dev)
+        for i in range(layers):
+            x = kv[i, every, take:take + max(counts)]
+            new = c.append(i, x[:, :, 0], x[:, :, 1], counts=n, rows=sub)
+            o = c.attend(i, q[i, every, take].contiguous(), new, rows=sub)
+            kp, vp, _, _ = c.layer(i)
+            table = c.page_table[every]
+            ref, mag, _ = define(q[i, every, take], kp, vp, table, new.tolist())
+            close(o, ref, mag, D)
+            if take and budget is None:
+                with pytest.raises(AssertionError):         # as if the newest token were missing
+                    r, m, _ = define(q[i, every, take], kp, vp, table, (new - 1).tolist())
+                    close(o, r, m, D)
+                with pytest.raises(AssertionError):         # as if all weights were equal
+                    r, m, _ = define(q[i, every, take] * 0, kp, vp, table, new.tolist())
+                    close(o, r, m, D)
+                for j, b in enumerate(every):               # what lies in the slots is what was given
+                    t = torch.tensor(fed[b] + list(range(take, take + counts[j])), device=dev)
+                    where = [(int(table[j, s // page]), s % page) for s in range(len(t))]
+                    assert torch.equal(torch.stack([kp[p, :, r] for p, r in where]), kv[i, b, t, 0])
+                    assert torch.equal(torch.stack([vp[p, :, r] for p, r in where]), kv[i, b, t, 1])
+        c.advance(counts, new, at)
+        for j, b in enumerate(every):
+            fed[b] += range(take, take + counts[j])
+
+    step(0, [20, 11, 1])
+    for take in range(20, 26):
+        step(take, [1, 1, 1])
+    for take in range(26, 30):
+        step(take, [1, 1], rows)
+    for take in range(30, 36):
+        step(take, [1, 1, 1])
+    seen = [len(f) for f in fed]
+    assert c.seen.tolist() == seen
+    assert c.lengths.tolist() == [min(n, budget or n) for n in seen] == c._slots

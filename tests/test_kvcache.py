@@ -718,3 +718,38 @@ def test_pools_in_one_place_are_refused(dev):
     paged_attention(q, k, v, table, n, scores=both[:, 0], scores_out=both[:, 1])
     paged_attention(q, k, v, table, n, scores=both[:, 0], scores_out=both[:, 0])
     assert both[:, 0].any()
+
+
+@GPU
+@pytest.mark.parametrize("D,H,G,page,dtype,rows,longest,weights", [
+    (128, 16, 1, 7, BF, 1400, 40, False), (128, 16, 1, 100, HF, 56, 1000, False),
+    (64, 16, 1, 100, BF, 120, 900, True), (64, 16, 2, 7, HF, 62, 1700, False),
+    (256, 16, 1, 16, BF, 110, 250, False), (256, 16, 1, 33, HF, 27, 1000, True),
+    (128, 16, 1, 64, HF, 130, 400, True), (64, 16, 3, 64, BF, 62, 1700, True), (256, 16, 2, 64, HF, 27, 1000, False),
+    (128, 4, 17, 16, BF, 210, 1000, False), (128, 4, 32, 5, HF, 210, 1000, False), (64, 4, 20, 16, BF, 420, 1000, True),
+    (256, 4, 17, 100, BF, 110, 1000, False), (128, 16, 1, 7, FL, 56, 500, False), (64, 16, 1, 20, FL, 56, 900, True),
+])
+def test_16_bits_streamed_past_the_caches(gpu, D, H, G, page, dtype, rows, longest, weights):
+    """Every form that takes its keys and values past the caches: head widths, pages of a multiple of 16 rows or of any size,
+    one work item to a sequence or several, one or two blocks of query heads, weights gathered or not."""
+    lengths = [longest - i % 7 for i in range(rows)]
+    assert 2 * H * D * torch.finfo(dtype).bits // 8 * sum(lengths) > 4e8
+    width = -(-longest // page)
+    g = torch.Generator("cuda").manual_seed(3)
+    k, v = (torch.randn(rows * width, H, page, D, generator=g, device="cuda", dtype=dtype) for _ in range(2))
+    table = torch.arange(rows * width, dtype=torch.int32, device="cuda").view(width, rows).t().contiguous()
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    q = torch.randn(rows, H * G, D, generator=g, device="cuda", dtype=dtype)
+    s = torch.zeros(k.shape[:3], device="cuda") if weights else None
+    o = paged_attention(q, k, v, table, n, scores=s)
+    for b in (0, rows // 2, rows - 1):
+        m = lengths[b]
+        own = table[b].long()
+        kb, vb = (t[own].transpose(0, 1).reshape(H, -1, D)[:, :m].double().cpu() for t in (k, v))
+        w = torch.softmax(q[b].double().cpu().view(H, G, D) @ kb.transpose(1, 2) / math.sqrt(D), -1)
+        close(o[b], (w @ vb).view(H * G, D), (w @ vb.abs()).view(H * G, D), D)
+        if weights:
+            got = s[own].transpose(0, 1).reshape(H, -1).double().cpu()
+            assert not got[:, m:].any()
+            want = w.sum(1)
+            assert ((got[:, :m] - want).abs() <= (2.0 ** -24 * 40 * (D + 3) + 2.0 ** -23) * want).all()
