@@ -244,6 +244,9 @@ class PagedKVCache:
         if evict:
             self.evict(rows)
 
+    def _kept_pages(self):
+        return min(self.page_table.shape[1], -(-(self.budget + self.slack + 1) // self.page))
+
     def _cut(self, n):
         return self.budget if n > self.budget + self.slack else n
 
@@ -255,14 +258,16 @@ class PagedKVCache:
             self.not_captured("an eviction from some rows")
         if self.budget is None or max((self._slots[x] for x in r), default=0) <= self.budget + self.slack:
             return
-        at = slice(None) if rows is None else r
-        self.lengths[at] = paged_evict(self.k, self.v, self.scores, self.positions, self._table()[at], self.lengths[at],
+        at, keep = slice(None) if rows is None else r, self._kept_pages()
+        # a table of the pages that rows own in the steady state: one of all pages would make a captured eviction slow
+        table = self.page_table[:, :keep] if _capturing(self.k) else self._table()
+        self.lengths[at] = paged_evict(self.k, self.v, self.scores, self.positions, table[at], self.lengths[at],
                                        self.seen[at], self.budget, self.recent, slack=self.slack)
+        if _capturing(self.k):      # the eviction leaves rows alone that are longer than its table
+            self._slots = [n if n > keep * self.page else self._cut(n) for n in self._slots]
+            return
         for x in r:
             self._slots[x] = self._cut(self._slots[x])
-        if _capturing(self.k):
-            return
-        keep = -(-(self.budget + self.slack + 1) // self.page)
         for x in r:
             own = self._pages[x]
             if len(own) > keep:
@@ -272,11 +277,18 @@ class PagedKVCache:
 
     def replayed(self, tokens=1, evicts=False):
         """Tells the host's book that a captured step, which gave every row ``tokens`` tokens and ended with an eviction
-        if ``evicts``, was replayed; the capture itself has been counted, as the first replay."""
+        if ``evicts`` (as it does if a row was past budget + slack when it was captured), was replayed; the capture itself
+        has been counted, as the first replay. A capture of several steps counts once for each. A captured eviction leaves
+        out rows that are more than a page past budget + slack, such as new prompts: they are cut down here."""
         slots = [n + tokens for n in self._slots]      # in use before the eviction
         if any(n > len(own) * self.page for n, own in zip(slots, self._pages)):
             raise RuntimeError("PagedKVCache: the replayed step ran past the pages that were reserved for it")
-        self._slots = [self._cut(n) for n in slots] if evicts else slots
+        self._slots = slots
+        if evicts:
+            most = self._kept_pages() * self.page
+            self._slots = [n if n > most else self._cut(n) for n in slots]
+            if max(slots) > most:
+                self.evict([r for r, n in enumerate(slots) if n > most])
 
 
 # ---------------------------------------------------------------------------- PyTorch implementation

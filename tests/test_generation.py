@@ -556,3 +556,79 @@ def test_attention_over_the_cache_against_64_bits(dev, D, page, budget):
     seen = [len(f) for f in fed]
     assert c.seen.tolist() == seen
     assert c.lengths.tolist() == [min(n, budget or n) for n in seen] == c._slots
+
+
+def test_a_captured_eviction_sees_the_pages_of_the_steady_state(monkeypatch):
+    """A table of all pages would cost a captured eviction what rows of max_length do. Rows past it are cut by replayed()."""
+    import zoo.ops.kvcache as kvcache
+    widths = []
+    real = kvcache.paged_evict
+    monkeypatch.setattr(kvcache, "paged_evict", lambda *a, **kw: widths.append(a[4].shape) or real(*a, **kw))
+    t = layer("cpu", blocks=1)
+    tok, pos = ids(3, 40, "cpu")
+    c = t.init_cache(3, max_length=200, page=4, budget=8, recent=2, slack=1)
+    t.prefill([tok[:, :20], pos[:, :20]], c, counts=[20, 9, 12])
+    c.reserve(1)
+    with monkeypatch.context() as m:
+        m.setattr(kvcache, "_capturing", lambda x: True)
+        t.decode([tok[:, 20], pos[:, 20]], c)
+    assert widths == [(3, 3)] and c._slots == [21, 8, 13] == c.lengths.tolist()
+    for step in range(2):       # a replay: rows 1 and 2 take a token each, by hand as the graph would do it
+        c.reserve(1)
+        c.lengths += 1
+        c.seen += 1
+        with monkeypatch.context() as m:
+            m.setattr(kvcache, "_capturing", lambda x: True)
+            slots, c._slots = c._slots, [n + 1 for n in c._slots]
+            c.evict()
+            c._slots = slots
+        c.replayed(1, evicts=True)
+        assert c._slots == [[8, 9, 8], [9, 8, 9]][step] == c.lengths.tolist()
+    assert all(len(own) <= 3 for own in c._pages)
+
+
+@pytest.mark.gpu
+def test_captured_step_with_a_budget_and_rows_that_come_and_go(gpu):
+    """Prompts past the budget in rows that were released: the replays and replayed() leave what eager steps leave."""
+    t = layer("cuda", blocks=2)
+    tok, pos = ids(3, 80, "cuda")
+    caches = [t.init_cache(3, max_length=120, page=4, budget=10, recent=3, slack=2) for _ in range(2)]
+    for c in caches:
+        t.prefill([tok[:, :14], pos[:, :14]], c)
+        t.decode([tok[:, 14], pos[:, 14]], c)
+        for i in (15, 16):
+            t.decode([tok[:, i], pos[:, i]], c)
+    eager, static = caches
+    assert eager._slots == [12] * 3
+    x, p = tok[:, 17].clone(), pos[:, 17].clone()
+    static.reserve(1)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = t.decode([x, p], static)
+    g.replay()
+    assert torch.equal(y, t.decode([x, p], eager))
+    at = [18, 18, 18]
+    for i in range(30):
+        if i in (3, 20):
+            b = 1 if i == 3 else 2
+            for c in caches:
+                c.release([b])
+                t.prefill([tok[b:b + 1, :41 + i], pos[b:b + 1, :41 + i]], c, rows=[b])
+            at[b] = 41 + i
+        x.copy_(torch.stack([tok[b, at[b]] for b in range(3)]))
+        p.copy_(torch.stack([pos[b, at[b]] for b in range(3)]))
+        static.reserve(1)
+        g.replay()
+        static.replayed(1, evicts=True)
+        want = t.decode([x, p], eager)
+        at = [n + 1 for n in at]
+        assert torch.equal(y, want), i
+        assert static.lengths.tolist() == eager.lengths.tolist() == eager._slots == static._slots
+        assert static.seen.tolist() == eager.seen.tolist() == at
+        assert [len(own) for own in static._pages] == [len(own) for own in eager._pages]
+    for b in range(3):
+        for s in range(eager._slots[b]):
+            e, f = int(eager.page_table[b, s // 4]), int(static.page_table[b, s // 4])
+            assert torch.equal(eager.positions[e, :, s % 4], static.positions[f, :, s % 4])
+            assert torch.equal(eager.k[e, :, s % 4], static.k[f, :, s % 4])
