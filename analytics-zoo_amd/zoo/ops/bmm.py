@@ -79,7 +79,7 @@ def matmul(a, b):
     if a.dim() < 2 or b.dim() < 2 or (a.dim() == 2 and b.dim() == 2) or not _right_in_rows(b):
         return torch.matmul(a, b)
     if b.dim() == 2:        # one plain product of all rows
-        return torch.matmul(a.reshape(-1, a.shape[-1]), b).reshape(*a.shape[:-1], b.shape[-1])
+        return torch.matmul(a.flatten(0, -2), b).reshape(*a.shape[:-1], b.shape[-1])
     return _MatmulFn.apply(a, b)
 
 

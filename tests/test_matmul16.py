@@ -76,6 +76,15 @@ def test_one_dimension_is_left_to_torch(as_on_gpu):
         bmm_module.matmul(a, b[:3])
 
 
+@pytest.mark.parametrize("sa,sb", [((4, 5, 0), (0, 3)), ((4, 5, 0), (4, 0, 3)), ((0, 5, 7), (7, 3)), ((4, 0, 7), (7, 0))])
+def test_nothing_to_sum_or_to_return(as_on_gpu, sa, sb):
+    a, b = torch.ones(sa).to(BF).requires_grad_(), torch.ones(sb).to(BF).requires_grad_()
+    c = bmm_module.matmul(a, b)
+    assert torch.equal(c, torch.matmul(a, b)) and not c.any()
+    c.sum().backward()
+    assert a.grad.shape == a.shape and b.grad.shape == b.shape
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("causal,mask", [(True, None), (False, (2, 1, 5, 7)), (False, (1, 3, 1, 7))])
 def test_plain_attention_forms_no_such_product(as_on_gpu, dtype, causal, mask):
