@@ -3292,8 +3292,8 @@ torch::Tensor paged_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, t
   }
   TORCH_CHECK(k.size(1) == v.size(1), what, ": k and v have other numbers of tokens");
   const int64_t T = k.size(1), vec = c.D * c.es / 16;
-  TORCH_CHECK(T * c.H * vec < (1LL << 31) - 256 && c.B * ((T * c.H * vec + 255) / 256 + 1) < (1LL << 24), what,
-              ": too many tokens in one call");    // below 2^32 threads
+  TORCH_CHECK(T < zoo::kKvMaxSlots && T * c.H * vec < (1LL << 31) - 256 && c.B * ((T * c.H * vec + 255) / 256 + 1) < (1LL << 24), what,
+              ": too many tokens in one call");    // lengths below 2^31, below 2^32 threads
   paged_written(kp, vp, table);
   if (counts.has_value()) paged_ints(*counts, lengths, "counts", what);
   if (seen.has_value()) paged_ints(*seen, lengths, "seen", what);

@@ -367,6 +367,8 @@ def _append_ref(k, v, k_pages, v_pages, page_table, lengths, counts, seen, score
     if v.shape != k.shape or (H, D) != (k_pages.shape[1], k_pages.shape[3]) or B != page_table.shape[0] \
             or k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
         raise RuntimeError("paged_append: k and v must be [batch, tokens, kv_heads, dim] of the cache's type")
+    if T >= 2 ** 30:
+        raise RuntimeError("paged_append: too many tokens in one call")
     _apart(k_pages, v_pages)
     new = lengths.clone()
     page = k_pages.shape[2]

@@ -753,3 +753,13 @@ def test_16_bits_streamed_past_the_caches(gpu, D, H, G, page, dtype, rows, longe
             assert not got[:, m:].any()
             want = w.sum(1)
             assert ((got[:, :m] - want).abs() <= (2.0 ** -24 * 40 * (D + 3) + 2.0 ** -23) * want).all()
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+def test_more_tokens_than_a_sequence_can_have(dev):
+    """A length is below 2^31 after any call that is taken: up to 2^30 slots and fewer than 2^30 tokens."""
+    _, k, v, table, n = make(1, 1, 1, 8, 8, [3], BF, dev)
+    x = torch.zeros(1, 1, 1, 8, dtype=BF, device=dev).expand(1, 2 ** 30, 1, 8)
+    with pytest.raises(RuntimeError, match="too many tokens"):
+        paged_append(x, x, k, v, table, n)
+    assert n.tolist() == [3]
