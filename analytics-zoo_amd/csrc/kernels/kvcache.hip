@@ -33,8 +33,8 @@
 // chunks and, where weights are wanted, turns the stored products into sum_g w_gj.
 //
 // Measured on one MI355X (a large copy: 4.8 TB/s): 64 sequences of 16k slots, 8 kv heads of 128, 64 query heads, bf16:
-// 632 us, 6.8 TB/s; 24 of up to 8k, fp16: 78 us, 5.4 TB/s; one of 131k with weights: 102 us and 8 for the join, 4.9 TB/s;
-// 32 of up to 512, 12 heads of 64, with weights: 12 us, of which 5 are the chain of look-ups, loads and the epilogue that
+// 633 us, 6.8 TB/s; 24 of up to 8k, fp16: 78 us, 5.4 TB/s; one of 131k with weights: 111 us with the join, 4.9 TB/s;
+// 32 of up to 512, 12 heads of 64, with weights: 13 us, of which 5 are the chain of look-ups, loads and the epilogue that
 // a call over 77 slots takes alone.
 #include <math.h>
 
@@ -620,6 +620,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT != kF32 && !P16
       if (more) load_v(base + T::GRAIN, nt);
     }
   };
+  // Rows that were padded share cache lines with their neighbours, which a load past the caches reads again (16 heads, 64
+  // sequences, bf16: 80 dims, 4096 slots 240 us through the caches and 301 past them, 200 dims 578 and 718, 96 277 and 304;
+  // 16 dims, 16384 slots 355 and 351).
   if (!PAD && w.big)
     stream(std::bool_constant<!PAD>{});
   else
@@ -774,7 +777,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Pag
 
 // ---- append: one thread moves 16 bytes of a token's key row and of its value row ----
 // Bound by HBM: 16 prompts of up to 2048 tokens, 8 heads of 128, bf16: 144 MB in 28 us, 5.1 TB/s. Neighbouring threads take
-// the pieces, then the heads of a token, as a packed projection has them side by side; 32 single tokens: 3.3 us.
+// the pieces, then the heads of a token, as a packed projection has them side by side; 32 single tokens: 3.2 us.
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs a, int blocks_per_seq) {
   const int b = blockIdx.x / blocks_per_seq;
   const uint32_t i = (uint32_t)(blockIdx.x - b * blocks_per_seq) * 256 + threadIdx.x;
@@ -1116,7 +1119,8 @@ __global__ __launch_bounds__(NT) void paged_evict_select_kernel(const PagedEvict
 // Rows of more slots than one workgroup should take: the same selection with a row shared out in segments of
 // kEvictSeg, a launch for each step that needs all of the row before it. Histograms of a row add
 // up in memory (whole numbers, so in any order). 8 rows of 131k slots: 35 us in five launches, one workgroup each 590. The
-// whole eviction from 8 rows of 16384 slots takes 31 us so and 33 with a workgroup each, from 256 rows 127 and 85.
+// whole eviction from 8 rows of 16384 slots takes 31 us so and 33 with a workgroup each, from 256 rows 127 and 85: the
+// border, kEvictHeld, is where a row's keys stop fitting LDS beside a second workgroup, and suits few long rows, not many.
 // STEP 0 .. 2: the digits, 3: counts of each wave's stretch, 4: the lists.
 template <int STEP>
 __global__ __launch_bounds__(256) void paged_evict_long_kernel(const PagedEvictArgs a) {

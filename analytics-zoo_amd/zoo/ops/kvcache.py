@@ -83,7 +83,12 @@ def paged_evict(k_pages, v_pages, scores, positions, page_table, lengths, seen, 
     position, so no more rows move than have to. A sequence of up to ``budget + slack`` slots keeps them all. Returns the new
     lengths as a new tensor.
 
-    Scores and positions of the kept slots go to ``scores_out`` and ``positions_out``, by default where they were."""
+    Scores and positions of the kept slots go to ``scores_out`` and ``positions_out``, by default where they were.
+
+    The call takes ``8 * min(budget, capacity - budget)`` bytes of workspace for each sequence and kv head, and for tables
+    of more than 16384 slots ``4 * capacity`` and 24 KB more, of which the 24 KB are cleared. The capacity, what a row of the
+    table can name, also chooses the form of the kernels: pass a narrower view of a wide table (a sequence that is longer
+    than the view keeps all its slots)."""
     scores_out = scores if scores_out is None else scores_out
     positions_out = positions if positions_out is None else positions_out
     if k_pages.is_cuda:
@@ -105,7 +110,9 @@ class PagedKVCache:
 
     A row's pages are taken as it grows (:meth:`reserve`) and given back by :meth:`release`; ``pages`` bounds their
     number, by default ``batch`` sequences of ``max_length`` slots. With ``budget``, sequences longer than ``budget +
-    slack`` slots are cut down to ``budget`` after a step; their last ``recent`` tokens stay.
+    slack`` slots are cut down to ``budget`` after a step of theirs; their last ``recent`` tokens stay. ``recent`` is 0 by
+    default: give some, or a new token competes with slots that have gathered weight for longer. Weight is gathered by
+    :meth:`attend`, so the slots of a prompt start with none, and its first eviction goes by the step before it.
 
     A step of every layer: :meth:`append`, :meth:`attend` per layer, then :meth:`advance`.
 

@@ -168,7 +168,7 @@ class TransformerLayer(Layer):
     def init_cache(self, batch, max_length=None, page=64, pages=None, budget=None, recent=None, slack=0):
         """A :class:`zoo.ops.PagedKVCache` for up to ``batch`` sequences of ``max_length`` (default: the layer's
         sequence length) slots. With ``budget`` a sequence keeps that many slots per head, the last ``recent`` tokens
-        and those that gathered the most attention."""
+        (default 0) and those that gathered the most attention in the decoding steps; prompts gather none."""
         max_length = self.seq_len if max_length is None else max_length
         if max_length is None:
             raise ValueError("init_cache: max_length is needed for a layer without a sequence length")
@@ -198,7 +198,7 @@ class TransformerLayer(Layer):
         """The prompts ``xs`` = [token_ids, position_ids] ([n, T]) into ``cache``: as rows ``rows`` (a list of n row
         numbers), which must be empty, all by default. ``counts`` (a list): how many tokens of each prompt are real,
         the rest is padding behind them. Returns the sequence output [n, T, hidden], as the layer's own call
-        does."""
+        does. Nothing is evicted before a row's first step of :meth:`decode`."""
         n, T = xs[0].shape
         at = cache.rows(rows)
         counts = [T] * n if counts is None else [int(c) for c in counts]
@@ -228,7 +228,8 @@ class TransformerLayer(Layer):
     @torch.no_grad()
     def decode(self, xs, cache, rows=None):
         """One token of every row of ``cache``, or of the rows ``rows`` (a list of numbers): ``xs`` = [token_ids,
-        position_ids] ([n]). Returns the sequence output of these tokens [n, hidden]."""
+        position_ids] ([n]). Returns the sequence output of these tokens [n, hidden]. Steps of every row can be captured
+        (:class:`zoo.ops.PagedKVCache`)."""
         at = cache.rows(rows)
         n = len(at)
         if n == 0 or xs[0].dim() != 1 or xs[0].shape[0] != n:
