@@ -228,12 +228,11 @@ ZOO_DEV f32x4 mma16(const uint4& x, const uint4& y, const f32x4& c) {
                                                   0);
 }
 
-// Weights are held times this. Sums of up to 2^30 weighted values stay finite even for the type's largest values
-// (bfloat16 and float32: 2^-32), and float16 parts hold weights down to 2^-38 of the wave's largest (2^15, below its 65504).
-template <int DT>
-constexpr float kWeight = DT == kF16 ? 0x1p15f : 0x1p-32f;
-template <int DT>
-constexpr float kWeightLog = DT == kF16 ? 15.f : -32.f;
+// Weights of a sequence of len slots are held times 2 to the power of this. In bfloat16 and float32 it is the first power
+// below 1 / len, so that sums of the type's largest values stay finite and those of small ones keep their bits; in
+// float16, whose values are far from the ends of float32's range, 2^15 (below its 65504): its parts then hold weights down
+// to 2^-38 of the wave's largest.
+ZOO_DEV int weight_log(int dt, int len) { return dt == kF16 ? 15 : __clz(len) - 32; }
 
 ZOO_DEV uint32_t high16(float x, float y) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); }
 // the upper 16 bits of the float next to x on the side of zero; of 0 for 0
@@ -373,6 +372,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT != kF32 && !P16
   const int gb = min(W, a.G - W * w.hb), D = a.D;
   const int head0 = w.hk * a.G + W * w.hb;
   const long out0 = ((long)w.b * a.H * a.G + head0) * D;
+  const int up = weight_log(DT, w.len);
+  const float up2 = __uint_as_float((uint32_t)(127 + up) << 23);
   if (w.len <= 0) {
     const float x = w.len < 0 ? __builtin_nanf("") : 0.f;
     for (int i = threadIdx.x; i < gb * D; i += 256) store_out<DT>(a.o, out0 + i, x);
@@ -560,7 +561,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT != kF32 && !P16
         for (int u = 0; u < NS; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            s[n][u][r] = pow2(s[n][u][r] - mu) * kWeight<DT>;
+            s[n][u][r] = pow2(s[n][u][r] - mu) * up2;
             l[n] += s[n][u][r];
           }
       }
@@ -680,7 +681,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : NB == 2 || (DT != kF32 && !P16
         a.part_ml[((long)item_of(a) * W + g) * 2] = bad_page ? __builtin_nanf("") : top;
         a.part_ml[((long)item_of(a) * W + g) * 2 + 1] = sum;
       }
-      lse[g] = bad_page ? kBadLse : top + log2f(sum) - kWeightLog<DT>;
+      lse[g] = bad_page ? kBadLse : top + log2f(sum) - up;
     }
   }
   if (weights) {
@@ -735,7 +736,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Pag
       bad_page = __ballot(bad_page) >> (tid & 48) & 0xffff;   // of the 16 threads of this head
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) merge(m, l, x, __shfl_xor(m, o, 64), __shfl_xor(l, o, 64), 0.f);
-      if (g < a.G && (tid & 15) == 0) lse[g] = bad_page ? kBadLse : m + log2f(l) - (a.dtype == kF16 ? kWeightLog<kF16> : kWeightLog<kF32>);
+      if (g < a.G && (tid & 15) == 0) lse[g] = bad_page ? kBadLse : m + log2f(l) - weight_log(a.dtype, w.len);
     }
     if (w.n == 1) __syncthreads();
   }

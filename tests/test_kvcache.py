@@ -763,3 +763,34 @@ def test_more_tokens_than_a_sequence_can_have(dev):
     with pytest.raises(RuntimeError, match="too many tokens"):
         paged_append(x, x, k, v, table, n)
     assert n.tolist() == [3]
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("dtype", [BF, FL])
+@pytest.mark.parametrize("scale", [2.0 ** -96, 2.0 ** 110])
+@pytest.mark.parametrize("n,width", [(45, None), (700, None), (900, 400)])
+def test_values_of_any_size(dev, dtype, scale, n, width):
+    """Outputs are as exact for tiny and for huge values: sums of 900 weighted values of 2^-96 stay above 2^-126 by more than
+    the 24 bits of their terms' largest, and of 2^110 below 2^128. Terms below 2^-126 are off by 2^-149 each, which is below
+    900 2^-149 2^96 < 2^-43 of the scale."""
+    q, k, v, table, lens = make(2, 2, 2, 64, 16, [n, 3], FL, dev, junk=0.0, width=width)
+    q, k, v = q.to(dtype), k.to(dtype), (v * scale).to(dtype)
+    ref, mag, _ = define(q, k, v, table, [n, 3])
+    o = paged_attention(q, k, v, table, lens).double().cpu()
+    tol = torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -24 * 40 * 67 * mag + 2.0 ** -43 * scale
+    assert ((o - ref).abs() <= tol).all(), ((o - ref).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("dtype", [BF, FL])
+@pytest.mark.parametrize("scale", [2.0 ** -96, 2.0 ** 110])
+def test_weights_are_kept_to_float32_for_values_of_any_size(dev, dtype, scale):
+    """As test_weights_are_kept_to_float32: scaling by a power of two changes no rounding of normal numbers, and what the two
+    slots give is above 2^-126 by 2^20 at least (values of 2^-4 of the scale and more) or moves the output by 2^-149, which is
+    2^-53 of the scale."""
+    q, k, v, table, n = _cancelling("cpu", dtype)
+    v = (v.double() * scale).to(dtype)
+    ref, mag, _ = define(q, k, v, table, [2] * 64, scale=1.0)
+    o = paged_attention(*(t.to(dev) for t in (q, k, v, table, n)), scale=1.0).double().cpu()
+    tol = torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -20 * mag + 2.0 ** -50 * scale
+    assert ((o - ref).abs() <= tol).all(), ((o - ref).abs() / tol).max().item()
