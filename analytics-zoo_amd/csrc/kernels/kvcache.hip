@@ -240,7 +240,8 @@ ZOO_DEV float below16(float x) { return __uint_as_float(__builtin_elementwise_su
 
 // Two weights as packed 16-bit numbers whose sum they are. Each part is cut off so that something is left for the
 // next one: an infinite value times a weight is then infinite in every part, where a part of 0 would make it NaN.
-// Only a weight of 0 has parts of 0.
+// Only a weight of 0 has parts of 0, or one so small that its parts leave the type's range (held in float16 below 2^-23, in
+// bfloat16 below 2^-102).
 // bfloat16: 8 bits in each of three parts, nothing is lost. float16: 11 bits in each of two, an error of 2^-22 of the weight
 // and 2^-25 (2^-40 of the wave's largest weight, in either direction, with no sign to add up in); what is below 2^-23
 // goes into the second part alone.

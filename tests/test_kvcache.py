@@ -794,3 +794,26 @@ def test_weights_are_kept_to_float32_for_values_of_any_size(dev, dtype, scale):
     o = paged_attention(*(t.to(dev) for t in (q, k, v, table, n)), scale=1.0).double().cpu()
     tol = torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -20 * mag + 2.0 ** -50 * scale
     assert ((o - ref).abs() <= tol).all(), ((o - ref).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=GPU)])
+@pytest.mark.parametrize("dtype,least", [(BF, -50.0), (HF, -25.0), (FL, -80.0)])
+def test_infinite_values_with_little_weight(dev, dtype, least):
+    """An infinite value comes through whatever the bits of its weight, down to exp(least): every part of a weight that is
+    split is above 0. With a weight of 0 it is NaN, as 0 times infinity is."""
+    g = torch.Generator().manual_seed(3)
+    q, k, v, table, n = make(64, 4, 1, 64, 16, [2] * 64, FL, "cpu", seed=1)
+    q.zero_()
+    q[:, :, 0] = 1.0
+    a = torch.rand(64, 4, generator=g) * least
+    a[0, 0] = -1000.0
+    for b in range(64):
+        p = int(table[b, 0])
+        k[p, :, :2] = 0.0
+        k[p, :, 1, 0] = a[b]
+        v[p, :, 1] = math.inf
+        v[p, 2:, 1] = -math.inf
+    o = paged_attention(*(t.to(dtype).to(dev) for t in (q, k, v)), table.to(dev), n.to(dev), scale=1.0).float().cpu()
+    assert torch.isnan(o[0, 0]).all()
+    o[0, 0] = math.inf
+    assert (o[:, :2] == math.inf).all() and (o[:, 2:] == -math.inf).all()
